@@ -272,7 +272,8 @@ def _fork(s):
     B, K = parents.shape
     whole, rest = s["case"]["length"] // PAGE, s["case"]["length"] % PAGE
     row = torch.arange(B, device=table.device)[:, None] * K + parents
-    old = table[row.view(-1)]
+    held = whole + (rest > 0)                     # columns behind the last held page are every row's own
+    old = table[row.view(-1), :held]
     if rest:
         tail = table[:, whole].long()
         same = parents[:, :, None] == parents[:, None, :]
@@ -283,7 +284,7 @@ def _fork(s):
         old[take, whole] = spare[take].int()
         spare = spare.clone()
         spare[take] = tail[give]
-    table.copy_(old)
+    table[:, :held] = old
     s["spare"].copy_(spare)
     return {"pools": pools, "table": table, "spare": s["spare"]}
 
