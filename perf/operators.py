@@ -189,7 +189,7 @@ def _seen(t):
 def _place(s):
     """Puts a state's inputs into tensors of the framework, with the outputs that a program keeps from call to call."""
     import kandle_b200
-    from kandle_b200 import core
+    from kandle_b200 import core, paged
 
     backend = kandle_b200.init(0)
     c, d = s["case"], {}
@@ -205,7 +205,7 @@ def _place(s):
         B, K = c["batch"], c["beams"]
         d.update(next=core.empty((B, K)), parents=core.empty((B, K), "int32"), tokens=core.empty((B, K), "int64"), ended=core.empty((B, K)))
     else:
-        d["list"] = [d["pools"].select(0, i) for i in range(2 * c["layers"])]
+        d["list"] = paged.Pools([d["pools"].select(0, i) for i in range(2 * c["layers"])])
     torch.cuda.synchronize()
     s["d"] = d
     s["out"] = {"attend": lambda: _seen(d["out"]), "beams": lambda: {n: _seen(d[n]) for n in ("next", "parents", "tokens", "ended")},
