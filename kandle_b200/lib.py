@@ -149,6 +149,10 @@ _SIGNATURES = {
     "kd_qkv_norm_rope_cachewrite_paged": [_T, _T, _T, ctypes.c_float, _T, _T, _T, _T, _T, _T, ctypes.c_int, _T],
     "kd_kv_pages_write": [_T, _T, _T, _T, _T, ctypes.c_int],
     "kd_qkv_linear_norm_rope_cachewrite": [_T, _T, _T, _T, ctypes.c_float, _T, _T, _T, _T, ctypes.c_int, _T],
+    "kd_attention_paged": [_T] * 6 + [ctypes.c_int, ctypes.c_float, _T],
+    "kd_kv_pages_copy": [_REFS, ctypes.c_int, _T, _T],
+    "kd_kv_pages_fork": [_REFS, ctypes.c_int] + [_T] * 4,
+    "kd_beam_select": [_T, _T, ctypes.c_int] + [_T] * 4,
     "kd_swiglu": [_T, _T],
     "kd_add_rmsnorm": [_T, _T, _T, ctypes.c_float, _T, _T],
     "kd_increment_i32": [_T, ctypes.c_int],

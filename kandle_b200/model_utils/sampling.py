@@ -64,3 +64,17 @@ def sample(logits: Tensor, config: SamplerConfig | None = None, displayTopK: int
 
 def sampleGreedy(logits: Tensor, displayTopK: int = 0) -> SampleResult:    # index.ts:243-248
     return sample(logits, SamplerConfig(doSample=False), displayTopK)
+
+
+def beam_select(logits: Tensor, scores: Tensor, eos: int = -1, out=None):
+    """One step of beam search for every request (kd_beam_select).  logits fp32 [requests, beams, V] (or [requests * beams, V]), scores
+    fp32 [requests, beams]: the log-probability of each beam so far.  Returns (scores, parents, tokens, ended), each [requests, beams]:
+    the best continuations that go on, best first (score, the beam that each continues, its token), and for every old beam the score with
+    which it ends here by `eos` if that is among the best as many as there are beams, else -inf.  out: tensors to write them to.
+    The reference has greedy and sampled tokens only."""
+    if out is None:
+        shape = scores.shape
+        out = tuple(Tensor(_handle=core._output(shape, dt)) for dt in ("float32", "int32", "int64", "float32"))
+    new, parents, tokens, ended = out
+    lib.call("kd_beam_select", _r(logits), _r(scores), int(eos), _r(new), _r(parents), _r(tokens), _r(ended))
+    return out
