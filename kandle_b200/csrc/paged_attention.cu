@@ -4,8 +4,11 @@
 // token i sees positions 0 .. ctx_b - n_b + i.
 #include "common.cuh"
 #include "kernels.cuh"
+#include "sm100.cuh"
 
 namespace kd {
+
+using namespace sm100;
 
 struct PagedParams {
   int T, B, Hq, Hkv, D, max_pages, pages;
@@ -45,7 +48,7 @@ __global__ void __launch_bounds__(256) paged_attention_kernel(const PagedParams 
   const int lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z;
   const PagedSeq s = paged_seq(p, b);
   const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= s.n) return;
+  if (i >= s.n || s.n * (p.Hq / p.Hkv) <= 64) return;
   const int hk = h / (p.Hq / p.Hkv), per = p.D / 32;
   float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -1e30f, l = 0.f;
   for (int e = 0; e < per; ++e) q[e] = __bfloat162float(p.q[(s.row0 + i) * p.sq_t + h * p.sq_h + lane * per + e]);
@@ -70,6 +73,464 @@ __global__ void __launch_bounds__(256) paged_attention_kernel(const PagedParams 
   for (int e = 0; e < per; ++e) p.o[(s.row0 + i) * p.so_t + h * p.so_h + lane * per + e] = __float2bfloat16_rn(o[e] * inv);
 }
 
+// ----------------------------------------------------------------------------- how the work is divided
+// Work of every KV head: per sequence `items` tiles of queries of `len` key tiles each.  An item is cut into parts of at most L key tiles,
+// and a block takes a part, so that long and short sequences fill the GPU alike.
+struct PagedWork {
+  int items, len;
+};
+constexpr int PA_CACHE = 512;       // sequences whose work is kept in shared memory while L is looked for
+constexpr int PA_FEW_ROWS = 64;     // rows (new tokens x query heads of a KV head) up to which a sequence is one item of the few-row kernel
+constexpr int PA_KEYS = 64;         // keys of a tile there
+
+__device__ __forceinline__ PagedWork few_work(const PagedParams& p, int b) {
+  const PagedSeq s = paged_seq(p, b);
+  const int rows = s.n * (p.Hq / p.Hkv);
+  if (rows == 0 || rows > PA_FEW_ROWS) return PagedWork{0, 0};
+  return PagedWork{1, (s.ctx + PA_KEYS - 1) / PA_KEYS};
+}
+__device__ __forceinline__ int parts_of(const PagedWork& w, int L) { return w.len <= L ? 1 : (w.len + L - 1) / L; }
+
+// What block x of a head does: part `part` of `parts` of item `item` of sequence b.  `place`: where the first part of the sequence's first item
+// leaves its sums, counted over the items that are cut (these have more than L tiles each, so there are at most `slots` of them and
+// 2 x `slots` parts).
+struct PagedPlan {
+  int b, item, part, parts, place;
+};
+// By one warp.  `slots`: blocks of a head that run at a time.  Returns b = -1 where there is no work for x.
+template <typename Work>
+__device__ __forceinline__ PagedPlan paged_plan(const PagedParams& p, Work work, int x, int slots, int least, int2* cache) {
+  const int lane = threadIdx.x & 31;
+  auto of = [&](int b) {
+    if (b < PA_CACHE) return PagedWork{cache[b].x, cache[b].y};
+    return work(p, b);
+  };
+  int64_t sum = 0;
+  int longest = 0;
+  for (int b = lane; b < p.B; b += 32) {
+    const PagedWork w = work(p, b);
+    if (b < PA_CACHE) cache[b] = make_int2(w.items, w.len);
+    sum += (int64_t)w.items * w.len;
+    longest = max(longest, w.len);
+  }
+  __syncwarp();
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  const int even = max(least, (int)((sum + slots - 1) / slots));
+  auto count = [&](int L) {
+    int n = 0;
+    for (int b = lane; b < p.B; b += 32) {
+      const PagedWork w = of(b);
+      n += w.items * parts_of(w, L);
+    }
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  // the smallest parts that run all at once; where that makes them a third longer than an even share, the even share
+  int L = even;
+  for (const int most = even + even / 3 + 1; L < longest && count(L) > slots;) {
+    L += max(1, L / 16);
+    if (L > most) {
+      L = even;
+      break;
+    }
+  }
+  PagedPlan plan{-1, 0, 0, 0, 0};
+  int before = 0, cut_before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const PagedWork w = b0 + lane < p.B ? of(b0 + lane) : PagedWork{0, 0};
+    const int parts = w.items ? parts_of(w, L) : 0, n = w.items * parts;
+    const int cut = parts > 1 ? n : 0;
+    int upto = n, cut_upto = cut;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o), u = __shfl_up_sync(0xffffffffu, cut_upto, o);
+      if (lane >= o) { upto += v; cut_upto += u; }
+    }
+    const int first = before + upto - n;
+    const unsigned hit = __ballot_sync(0xffffffffu, x >= first && x < first + n);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      plan.b = b0 + who;
+      plan.parts = __shfl_sync(0xffffffffu, parts, who);
+      plan.place = __shfl_sync(0xffffffffu, cut_before + cut_upto - cut, who);
+      const int at = x - __shfl_sync(0xffffffffu, first, who);
+      plan.item = at / plan.parts;
+      plan.part = at % plan.parts;
+      return plan;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    cut_before += __shfl_sync(0xffffffffu, cut_upto, 31);
+  }
+  return plan;
+}
+
+// ----------------------------------------------------------------------------- few query rows: one pass over the keys at HBM speed
+// The rows of a sequence and KV head (its new tokens times the query heads on it, at most 64) are one tile.  Keys and values come as tiles of 64
+// through a ring of TMA copies.  Four groups of warps each take 16 keys of a tile, with a running maximum and sum of their own, so that
+// no warp waits for another before the end; there they are joined in shared memory.  Tiles of 16 rows suit mma.sync (m16n8k16): with 2 to
+// 16 live rows a tcgen05 tile of 128 would compute eight times as much and leave its softmax to as many threads.  Bound: HBM.
+struct PagedSplit {
+  float* part_o;      // [part][Hkv][rows][D] unnormalised sums
+  float2* part_ml;    // [part][Hkv][rows] (running maximum in the log2 domain, sum)
+  int2* plan;         // per sequence: place of its first part, parts of an item
+  int slots;
+};
+
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// MT tiles of 16 rows a warp, RG groups of warps side by side over the rows.
+template <int D, int MT, int RG>
+struct FewShape {
+  static constexpr int ROWS = 16 * MT * RG, WARPS = 4 * RG, THREADS = 32 * (WARPS + 1);
+  static constexpr int TILE = PA_KEYS * D * 2, CTAS = RG == 1 ? 2 : 1;
+  static constexpr int SLOTS = (CTAS == 2 ? 96 : 192) * 1024 / TILE;
+  static constexpr int Q_BYTES = ROWS * D * 2;
+  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * TILE + SLOTS * 16 + ROWS * 4 * 8 + 64;
+  static_assert(4 * ROWS * D * 4 <= SLOTS * TILE, "the warps' sums are joined in the ring");
+};
+
+template <int D, int MT, int RG>
+__global__ void __launch_bounds__(FewShape<D, MT, RG>::THREADS, FewShape<D, MT, RG>::CTAS)
+paged_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PagedParams p, const PagedSplit out) {
+  using S = FewShape<D, MT, RG>;
+  constexpr int SLAB = PA_KEYS * 128, QSLAB = S::ROWS * 128, NT = D / 8;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int2 cache[PA_CACHE];
+  __shared__ PagedPlan plan_s;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;
+  uint8_t* q_smem = ring + S::SLOTS * S::TILE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(q_smem + S::Q_BYTES);
+  uint64_t* empty = full + S::SLOTS;
+  float2* ml = reinterpret_cast<float2*>(empty + S::SLOTS);        // [key group][row]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ml + 4 * S::ROWS);      // and behind it one that stays 0
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y, group = p.Hq / p.Hkv;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::SLOTS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], S::WARPS); }
+    abort_flag[0] = abort_flag[1] = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+  }
+  pdl_wait();
+  if (warp == S::WARPS) {
+    const PagedPlan plan = paged_plan(p, few_work, blockIdx.x, out.slots, 2, cache);
+    if (lane == 0) {
+      plan_s = plan;
+      if (plan.b >= 0 && plan.part == 0 && hk == 0) out.plan[plan.b] = make_int2(plan.place, plan.parts);
+    }
+  }
+  __syncthreads();
+  const PagedPlan plan = plan_s;
+  if (plan.b < 0) return;
+  const PagedSeq s = paged_seq(p, plan.b);
+  const int rows = s.n * group, tiles = (s.ctx + PA_KEYS - 1) / PA_KEYS;
+  const int j0 = (int)((int64_t)tiles * plan.part / plan.parts), j1 = (int)((int64_t)tiles * (plan.part + 1) / plan.parts);
+  const int hidden = s.ctx - s.n;                                  // keys 0 .. hidden + i are seen by token i
+
+  int issued = 0;                                                  // by the copying warp
+  if (warp == S::WARPS) {
+    bool ok = true;
+    int page = 0;
+    for (int j = j0; ok && j < j1; ++j) {
+      const int i = j - j0;
+      // 32 entries of the table at a time
+      if (i % 64 == 0 || (j % 2 == 0 && (j / 2 - j0 / 2) % 32 == 0)) {
+        const int at = j / 2 + lane;
+        page = at < p.max_pages ? p.table[plan.b * p.table_row + at] : 0;
+        if (at <= (j1 - 1) / 2 && (unsigned)page >= (unsigned)p.pages && atomicCAS(p.err, 0, 103) == 0) { p.err[1] = plan.b; p.err[2] = page; }
+      }
+      const int where = __shfl_sync(0xffffffffu, page, (j / 2 - j0 / 2) % 32);
+      for (int kv = 0; kv < 2; ++kv) {
+        const int t = 2 * i + kv, slot = t % S::SLOTS;
+        ok = mbar_wait(&empty[slot], (uint32_t)(((t / S::SLOTS) & 1) ^ 1), abort_flag, p.err, 321);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full[slot], S::TILE);
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d) tma_load_4d(ring + slot * S::TILE + d * SLAB, kv ? &tmap_v : &tmap_k, &full[slot], d * 64, (j % 2) * 64, hk, where);
+        }
+        __syncwarp();
+        issued = t + 1;
+      }
+    }
+  } else {
+    // the rows of q, swizzled as the copies are
+    for (int i = threadIdx.x; i < S::ROWS * (D / 8); i += 32 * S::WARPS) {
+      const int r = i / (D / 8), c = i % (D / 8);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows) v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(s.row0 + r / group) * p.sq_t + (int64_t)(hk * group + r % group) * p.sq_h + c * 8);
+      *reinterpret_cast<uint4*>(q_smem + (c / 8) * QSLAB + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = v;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
+    const int kg = warp & 3, rg = warp >> 2, lr = lane & 7, mi = lane >> 3, row_a = lane >> 2, col = (lane & 3) * 2;
+    const int row0 = rg * 16 * MT;
+    const uint32_t q_base = smem_u32(q_smem), ring_base = smem_u32(ring);
+    auto q_frag = [&](uint32_t (&a)[4], int mt, int k) {
+      const int r = row0 + mt * 16 + (mi & 1) * 8 + lr, c = 2 * k + (mi >> 1);
+      ldsm4(a, q_base + (c / 8) * QSLAB + r * 128 + (((c % 8) ^ (r & 7)) << 4));
+    };
+    uint32_t qr[MT == 1 ? D / 16 : 1][4];
+    if constexpr (MT == 1) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) q_frag(qr[k], 0, k);
+    }
+    float o[MT][NT][4], m[MT][2], l[MT][2];
+    int last[MT][2];                                               // the last key that a row sees
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row0 + mt * 16 + h * 8 + row_a;
+        m[mt][h] = -1e30f;
+        l[mt][h] = 0.f;
+        last[mt][h] = r < rows ? hidden + r / group : -1;
+      }
+    }
+    bool ok = true;
+    for (int j = j0; j < j1; ++j) {
+      const int tk = 2 * (j - j0), sk = tk % S::SLOTS, sv = (tk + 1) % S::SLOTS;
+      ok = mbar_wait(&full[sk], (uint32_t)((tk / S::SLOTS) & 1), abort_flag, p.err, 322);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      float sc[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[mt][n][e] = 0.f;
+      {
+        const int key = kg * 16 + (mi >> 1) * 8 + lr;
+        const uint32_t base = ring_base + sk * S::TILE + key * 128;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const int c = 2 * k + (mi & 1);
+          uint32_t kb[4];
+          ldsm4(kb, base + (c / 8) * SLAB + (((c % 8) ^ (key & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t qa[4];
+            if constexpr (MT == 1) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) qa[e] = qr[k][e];
+            } else {
+              q_frag(qa, mt, k);
+            }
+            mma16(sc[mt][0], qa, kb[0], kb[1]);
+            mma16(sc[mt][1], qa, kb[2], kb[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[sk]);
+      const int key0 = j * PA_KEYS + kg * 16;
+      uint32_t pa[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if (key0 + 15 > hidden) {                                  // some token does not see all of these keys
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + n * 8 + col + (e & 1) > last[mt][e >> 1]) sc[mt][n][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(fmaxf(sc[mt][0][2 * h], sc[mt][0][2 * h + 1]), fmaxf(sc[mt][1][2 * h], sc[mt][1][2 * h + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float now = fmaxf(m[mt][h], mx * p.scale_log2);
+          const float a = pa_exp2(m[mt][h] - now);
+          m[mt][h] = now;
+          l[mt][h] *= a;
+          if (__any_sync(0xffffffffu, a != 1.f)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) { o[mt][n][2 * h] *= a; o[mt][n][2 * h + 1] *= a; }
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float e0 = pa_exp2(fmaf(sc[mt][n][2 * h], p.scale_log2, -now)), e1 = pa_exp2(fmaf(sc[mt][n][2 * h + 1], p.scale_log2, -now));
+            l[mt][h] += e0 + e1;
+            // probabilities meet the values as bf16, the type of the tensor cores' other operand; their sum stays in fp32
+            pa[mt][2 * n + h] = pack_bf16(e0, e1);
+          }
+        }
+      }
+      ok = mbar_wait(&full[sv], (uint32_t)(((tk + 1) / S::SLOTS) & 1), abort_flag, p.err, 323);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      if (j * PA_KEYS + PA_KEYS > s.ctx) {
+        // behind the last key the page may hold anything, and 0 x NaN is none: those values become zeros
+        for (int r = max(s.ctx - j * PA_KEYS, kg * 16); r < kg * 16 + 16; ++r)
+          for (int d = lane; d < D / 2; d += 32) *reinterpret_cast<uint32_t*>(ring + sv * S::TILE + (d / 32) * SLAB + r * 128 + (d % 32) * 4) = 0;
+        __syncwarp();
+      }
+      {
+        const int key = kg * 16 + (mi & 1) * 8 + lr;
+        const uint32_t base = ring_base + sv * S::TILE + key * 128;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          const int c = 2 * n + (mi >> 1);
+          uint32_t vb[4];
+          ldsm4_t(vb, base + (c / 8) * SLAB + (((c % 8) ^ (key & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16(o[mt][2 * n], pa[mt], vb[0], vb[1]);
+            mma16(o[mt][2 * n + 1], pa[mt], vb[2], vb[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[sv]);
+    }
+    // Join the key groups.  Every copy has landed and been read when all warps are here (a failed wait ends them all, and none is looked at).
+    float* sums = reinterpret_cast<float*>(ring);                  // [key group][row][D]
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row0 + mt * 16 + h * 8 + row_a;
+        float x = l[mt][h];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if ((lane & 3) == 0) ml[kg * S::ROWS + r] = make_float2(m[mt][h], x);
+        if (r < rows) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(sums + (kg * S::ROWS + r) * D + n * 8 + col) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+        }
+      }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
+    if (!*abort_flag) {
+      // 8 channels a thread
+      for (int i = threadIdx.x; i < rows * (D / 8); i += 32 * S::WARPS) {
+        const int r = i / (D / 8), c = i % (D / 8) * 8;
+        float w[4], M = -1e30f, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) M = fmaxf(M, ml[k * S::ROWS + r].x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = ml[k * S::ROWS + r];
+          w[k] = pa_exp2(x.x - M);
+          L += w[k] * x.y;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 a = *reinterpret_cast<const float4*>(sums + (k * S::ROWS + r) * D + c), e = *reinterpret_cast<const float4*>(sums + (k * S::ROWS + r) * D + c + 4);
+          acc[0] += w[k] * a.x; acc[1] += w[k] * a.y; acc[2] += w[k] * a.z; acc[3] += w[k] * a.w;
+          acc[4] += w[k] * e.x; acc[5] += w[k] * e.y; acc[6] += w[k] * e.z; acc[7] += w[k] * e.w;
+        }
+        if (plan.parts == 1) {
+          const float inv = L > 0.f ? 1.f / L : 0.f;               // a token that sees nothing gets a zero row
+          *reinterpret_cast<uint4*>(p.o + (int64_t)(s.row0 + r / group) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h + c) =
+              make_uint4(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv), pack_bf16(acc[4] * inv, acc[5] * inv), pack_bf16(acc[6] * inv, acc[7] * inv));
+        } else {
+          const int64_t at = ((int64_t)(plan.place + plan.part) * p.Hkv + hk) * S::ROWS + r;
+          float4* to = reinterpret_cast<float4*>(out.part_o + at * D + c);
+          to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+          if (c == 0) out.part_ml[at] = make_float2(M, L);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort_flag && warp == S::WARPS)                             // copies still on their way land before the block ends
+    for (int t = max(0, issued - S::SLOTS); t < issued; ++t) mbar_wait(&full[t % S::SLOTS], (uint32_t)((t / S::SLOTS) & 1), abort_flag + 1, p.err, 324);
+  pdl_trigger();
+}
+
+// Joins the parts of items that were cut: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A warp per token and head.
+template <int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p, const PagedSplit in, int part_rows) {
+  constexpr int W = D / 32;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, b = blockIdx.z, h = blockIdx.y, group = p.Hq / p.Hkv, i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const PagedSeq s = paged_seq(p, b);
+  if (i >= s.n || s.n * group > part_rows) return;
+  const int2 plan = in.plan[b];
+  if (plan.y <= 1) return;
+  const int hk = h / group, r = i * group + h % group;
+  auto place = [&](int k) { return ((int64_t)(plan.x + k) * p.Hkv + hk) * part_rows + r; };
+  float M = -1e30f;
+  for (int k = lane; k < plan.y; k += 32) M = fmaxf(M, in.part_ml[place(k)].x);
+  M = warp_max(M);
+  float L = 0.f, acc[W] = {};
+#pragma unroll 4
+  for (int k = 0; k < plan.y; ++k) {
+    const int64_t at = place(k);
+    const float2 x = in.part_ml[at];
+    const float w = x.y == 0.f ? 0.f : pa_exp2(x.x - M);
+    L += w * x.y;
+    const float* o = in.part_o + at * D + lane * W;
+#pragma unroll
+    for (int e = 0; e < W; ++e) acc[e] += w * o[e];
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  __nv_bfloat16* o = p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)h * p.so_h + lane * W;
+#pragma unroll
+  for (int e = 0; e < W; e += 2) *reinterpret_cast<__nv_bfloat162*>(o + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
+}
+
+template <int D, int MT, int RG>
+static int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p) {
+  using S = FewShape<D, MT, RG>;
+  static bool configured[64] = {false};   // per device: kd_shutdown + kd_init may move the library to another GPU
+  if (!configured[ctx().device & 63]) {
+    KD_CUDA_CHECK(cudaFuncSetAttribute(paged_few_kernel<D, MT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    configured[ctx().device & 63] = true;
+  }
+  PagedSplit out{};
+  out.slots = S::CTAS * ctx().sm_count / p.Hkv;
+  if (out.slots < 1) out.slots = 1;
+  const uint64_t places = 2 * (uint64_t)out.slots * p.Hkv * S::ROWS;
+  void* scratch;
+  KD_TRY(get_workspace(places * (D * 4 + 8) + (uint64_t)p.B * 8, &scratch));
+  out.part_o = static_cast<float*>(scratch);
+  out.part_ml = reinterpret_cast<float2*>(out.part_o + places * D);
+  out.plan = reinterpret_cast<int2*>(out.part_ml + places);
+  KD_CUDA_CHECK(launch_ex(paged_few_kernel<D, MT, RG>, dim3(out.slots + p.B, p.Hkv), dim3(S::THREADS), (size_t)S::SMEM, tk, tv, p, out));
+  KD_TRY(after_launch("paged_few_kernel"));
+  const int most = p.max_query * (p.Hq / p.Hkv) < S::ROWS ? p.max_query : S::ROWS / (p.Hq / p.Hkv);
+  KD_CUDA_CHECK(launch_ex(paged_join_kernel<D>, dim3((most + 7) / 8, p.Hq, p.B), dim3(256), 0, p, out, S::ROWS));
+  return after_launch("paged_join_kernel");
+}
+template <int D>
+static int few_rows(const kd_tensor* k_pool, const kd_tensor* v_pool, const PagedParams& p) {
+  CUtensorMap tk, tv;
+  KD_TRY(make_tmap_bhsd(&tk, p.k, k_pool->shape, k_pool->strides, PA_KEYS));
+  KD_TRY(make_tmap_bhsd(&tv, p.v, v_pool->shape, v_pool->strides, PA_KEYS));
+  const int64_t rows = (int64_t)p.max_query * (p.Hq / p.Hkv);
+  if (rows <= 16) return launch_few<D, 1, 1>(tk, tv, p);
+  if (rows <= 32) return launch_few<D, 2, 1>(tk, tv, p);
+  return launch_few<D, 2, 2>(tk, tv, p);
+}
+
 }  // namespace kd
 
 using namespace kd;
@@ -83,7 +544,7 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   KD_REQUIRE(q->shape[0] <= 0x7fffff00 && k_pool->shape[0] <= 0x7fffffff, "too many tokens or pages");
   const int T = (int)q->shape[0], Hq = (int)q->shape[1], D = (int)q->shape[2], Hkv = (int)k_pool->shape[1];
   KD_REQUIRE(D == 64 || D == 128, "head size %d: 64 or 128 are handled", D);
-  KD_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 64, "%d query heads on %d key heads: a multiple of them, up to 64 times, is handled", Hq, Hkv);
+  KD_REQUIRE(Hkv > 0 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0 && Hq / Hkv <= 64, "%d query heads on %d key heads: a multiple of them, up to 64 times, is handled", Hq, Hkv);
   KD_REQUIRE(k_pool->shape[2] == 128 && k_pool->shape[3] == D, "pools must be [pages,Hkv,128,%d]", D);
   for (int i = 0; i < 4; ++i) KD_REQUIRE(v_pool->shape[i] == k_pool->shape[i], "the pools' shapes differ");
   for (int i = 0; i < 3; ++i) KD_REQUIRE(out->shape[i] == q->shape[i], "out must have q's shape");
@@ -91,11 +552,12 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   for (int i = 0; i < 2; ++i) KD_REQUIRE(q->strides[i] % 8 == 0 && out->strides[i] % 8 == 0, "strides must be multiples of 8 elements");
   for (int i = 0; i < 3; ++i)
     KD_REQUIRE(k_pool->strides[i] % 8 == 0 && v_pool->strides[i] % 8 == 0 && k_pool->strides[i] >= 0 && v_pool->strides[i] >= 0, "strides must be multiples of 8 elements");
+  KD_REQUIRE(k_pool->shape[0] >= 1, "the pools hold no page");
   KD_REQUIRE(block_table->ndim == 2 && block_table->dtype == KD_I32 && block_table->strides[1] == 1 && block_table->strides[0] >= 0, "block_table must be int32 [B,max_pages] with rows in one piece");
   KD_REQUIRE(block_table->shape[0] <= 65535 && block_table->shape[1] < (1 << 24), "the block table is too large");
   const int B = (int)block_table->shape[0], max_pages = (int)block_table->shape[1];
   KD_REQUIRE(ctx_len->dtype == KD_I32 && is_contiguous(ctx_len) && (numel(ctx_len) == B || numel(ctx_len) == 1), "ctx_len must be int32 [B] or one number for all");
-  KD_REQUIRE(scale > 0.f && scale < 1e30f, "scale must be positive");
+  KD_REQUIRE(scale >= 1e-6f && scale <= 1e6f, "scale must lie between 1e-6 and 1e6");
   if (q_start) {
     KD_REQUIRE(q_start->dtype == KD_I32 && is_contiguous(q_start) && numel(q_start) == (int64_t)B + 1, "q_start must be int32 [B+1]");
   } else {
@@ -123,6 +585,10 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   for (int i = 0; i < 3; ++i) { p.sk[i] = k_pool->strides[i]; p.sv[i] = v_pool->strides[i]; }
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = ctx().error_flag;
-  KD_CUDA_CHECK(launch_ex(paged_attention_kernel, dim3((p.max_query + 7) / 8, Hq, B), dim3(256), 0, p));
-  return after_launch("paged_attention_kernel");
+  if ((int64_t)p.max_query * (Hq / Hkv) > PA_FEW_ROWS) {
+    KD_CUDA_CHECK(launch_ex(paged_attention_kernel, dim3((p.max_query + 7) / 8, Hq, B), dim3(256), 0, p));
+    KD_TRY(after_launch("paged_attention_kernel"));
+    if (!q_start) return KD_OK;
+  }
+  return D == 128 ? few_rows<128>(k_pool, v_pool, p) : few_rows<64>(k_pool, v_pool, p);
 }
