@@ -41,38 +41,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
   return s;
 }
 
-// One warp per query row and head.
-__global__ void __launch_bounds__(256) paged_attention_kernel(const PagedParams p) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z;
-  const PagedSeq s = paged_seq(p, b);
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= s.n || s.n * (p.Hq / p.Hkv) <= 64) return;
-  const int hk = h / (p.Hq / p.Hkv), per = p.D / 32;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -1e30f, l = 0.f;
-  for (int e = 0; e < per; ++e) q[e] = __bfloat162float(p.q[(s.row0 + i) * p.sq_t + h * p.sq_h + lane * per + e]);
-  const int seen = s.ctx - s.n + i + 1;
-  for (int j = 0; j < seen; ++j) {
-    const int page = p.table[b * p.table_row + j / 128];
-    if ((unsigned)page >= (unsigned)p.pages) {
-      if (lane == 0 && atomicCAS(p.err, 0, 103) == 0) { p.err[1] = b; p.err[2] = page; }
-      continue;
-    }
-    const __nv_bfloat16* k = p.k + page * p.sk[0] + hk * p.sk[1] + (j % 128) * p.sk[2] + lane * per;
-    const __nv_bfloat16* v = p.v + page * p.sv[0] + hk * p.sv[1] + (j % 128) * p.sv[2] + lane * per;
-    float d = 0.f;
-    for (int e = 0; e < per; ++e) d += q[e] * __bfloat162float(k[e]);
-    d = warp_sum(d) * p.scale_log2;
-    const float m2 = fmaxf(m, d), a = exp2f(m - m2), w = exp2f(d - m2);
-    for (int e = 0; e < per; ++e) o[e] = o[e] * a + w * __bfloat162float(v[e]);
-    l = l * a + w;
-    m = m2;
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;     // a token that sees nothing gets a zero row
-  for (int e = 0; e < per; ++e) p.o[(s.row0 + i) * p.so_t + h * p.so_h + lane * per + e] = __float2bfloat16_rn(o[e] * inv);
-}
-
 // ----------------------------------------------------------------------------- how the work is divided
 // Work of every KV head: per sequence `items` tiles of queries of `len` key tiles each.  An item is cut into parts of at most L key tiles,
 // and a block takes a part, so that long and short sequences fill the GPU alike.
@@ -88,6 +56,13 @@ __device__ __forceinline__ PagedWork few_work(const PagedParams& p, int b) {
   const int rows = s.n * (p.Hq / p.Hkv);
   if (rows == 0 || rows > PA_FEW_ROWS) return PagedWork{0, 0};
   return PagedWork{1, (s.ctx + PA_KEYS - 1) / PA_KEYS};
+}
+// Two tiles of 128 rows an item; a tile holds the query heads of as many tokens as fit.
+__device__ __forceinline__ PagedWork tile_work(const PagedParams& p, int b) {
+  const PagedSeq s = paged_seq(p, b);
+  const int group = p.Hq / p.Hkv, tokens = 2 * (128 / group);
+  if (s.n * group <= PA_FEW_ROWS) return PagedWork{0, 0};
+  return PagedWork{(s.n + tokens - 1) / tokens, (s.ctx + 127) / 128};
 }
 __device__ __forceinline__ int parts_of(const PagedWork& w, int L) { return w.len <= L ? 1 : (w.len + L - 1) / L; }
 
@@ -464,19 +439,366 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   pdl_trigger();
 }
 
-// Joins the parts of items that were cut: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A warp per token and head.
+// ----------------------------------------------------------------------------- many query rows: tcgen05
+// A block owns two tiles of 128 rows (a token's query heads side by side, so that a tile of 128 / group tokens shares every key of
+// their KV head) and passes over the pages of its part; a page is a key tile, found through the block table.
+//   warps 0-3   softmax and output of tile A, a row per thread      warps 4-7   the same for tile B
+//   warp 8      TMA: both query tiles, then the pages through two slots for keys and two for values
+//   warp 9      tcgen05.mma: QK_A(0) QK_B(0) | PV_A(j) QK_A(j+1) PV_B(j) QK_B(j+1) | ..., one tile's products beside the other's softmax
+//   warps 10-11 complete the third warpgroup, which hands registers to the softmax (72 against 216 a thread)
+// TMEM (512 columns): scores of A and B, overwritten by the probabilities as packed bf16, and both sums.  The running maximum is raised only
+// when it grew by more than 2^8.  Bound: the softmax's issued instructions beside the tensor pipe.
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// (x0, x1) = (a0, a1) * s + m
+__device__ __forceinline__ void pa_fma2(float& x0, float& x1, float a0, float a1, float s, float m) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(s), "f"(m));
+}
+// (s0, s1) += (a0, a1)
+__device__ __forceinline__ void pa_add2(float& s0, float& s1, float a0, float a1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
+}
+
+constexpr int PT_THREADS = 384, PT_ROWS = 256;
+
 template <int D>
+__global__ void __launch_bounds__(PT_THREADS, 1)
+paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                   const __grid_constant__ PagedParams p, const PagedSplit out) {
+  constexpr int SLABS = D / 64, NK = 2, NV = 2, TILE = 128 * D * 2, SLAB = 128 * 128;
+  constexpr uint32_t TMEM_COLS = 512;     // scores of tile t at 128 t, sums at 256 + D t
+  constexpr uint32_t IDESC_QK = make_idesc_bf16(128, 128, 0, 0), IDESC_PV = make_idesc_bf16(128, D, 0, 1);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int2 cache[PA_CACHE];
+  __shared__ PagedPlan plan_s;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = smem;
+  uint8_t* k_ring = q_smem + 2 * TILE;
+  uint8_t* v_ring = k_ring + NK * TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(v_ring + NV * TILE);
+  uint64_t* q_full = bars;          // 1
+  uint64_t* t_full = bars + 1;      // 4: key slots, then value slots
+  uint64_t* t_empty = bars + 5;     // 4
+  uint64_t* s_full = bars + 9;      // 2
+  uint64_t* p_ready = bars + 11;    // 4: [tile][half of the keys]
+  uint64_t* o_done = bars + 15;     // 2
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);     // and behind it one that stays 0
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y, group = p.Hq / p.Hkv, per_tile = 128 / group;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < NK + NV; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 1); }
+    for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&o_done[t], 1); }
+    for (int t = 0; t < 4; ++t) mbar_init(&p_ready[t], 4);
+    abort_flag[0] = abort_flag[1] = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+  }
+  pdl_wait();
+  if (warp == 8) {
+    const PagedPlan plan = paged_plan(p, tile_work, blockIdx.x, out.slots, 2, cache);
+    if (lane == 0) {
+      plan_s = plan;
+      if (plan.b >= 0 && plan.item == 0 && plan.part == 0 && hk == 0) out.plan[plan.b] = make_int2(plan.place, plan.parts);
+    }
+  }
+  __syncthreads();
+  const PagedPlan plan = plan_s;
+  if (plan.b < 0) return;
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();   // after the TMEM allocation (see common.cuh)
+
+  const PagedSeq s = paged_seq(p, plan.b);
+  const int hidden = s.ctx - s.n;                 // keys 0 .. hidden + i are seen by token i
+  // the last tokens, which see the most keys, begin first
+  const int items = (s.n + 2 * per_tile - 1) / (2 * per_tile), item = items - 1 - plan.item;
+  int tok0[2], nblk[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    tok0[t] = (2 * item + t) * per_tile;
+    nblk[t] = tok0[t] >= s.n ? 0 : (max(0, hidden + min(s.n, tok0[t] + per_tile)) + 127) / 128;
+  }
+  const int all = max(nblk[0], nblk[1]), j0 = (int)((int64_t)all * plan.part / plan.parts), n_blocks = (int)((int64_t)all * (plan.part + 1) / plan.parts) - j0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) nblk[t] = min(max(nblk[t] - j0, 0), n_blocks);     // block numbers below count from j0
+
+  int issued = 0;                                 // pages' keys and values by the copying warp
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  // whole warps wait and an elected lane issues (see attention_prefill2.cu)
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code)); };
+  if (warp == 8) {
+    if (n_blocks > 0) {
+      if (elect_one()) {
+        mbar_arrive_expect_tx(q_full, 2 * SLABS * per_tile * group * 128);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int d = 0; d < SLABS; ++d) tma_load_4d(q_smem + t * TILE + d * SLAB, &tmap_q, q_full, d * 64, hk * group, s.row0 + tok0[t], 0);
+      }
+      __syncwarp();
+      int page = 0;
+      for (int j = 0; j < n_blocks; ++j) {
+        if (j % 32 == 0) {       // 32 entries of the table at a time
+          page = j + lane < n_blocks ? p.table[plan.b * p.table_row + j0 + j + lane] : 0;
+          if ((unsigned)page >= (unsigned)p.pages && atomicCAS(p.err, 0, 103) == 0) { p.err[1] = plan.b; p.err[2] = page; }
+        }
+        const int where = __shfl_sync(0xffffffffu, page, j % 32);
+        if (!wait(&t_empty[j % NK], (uint32_t)(((j / NK) & 1) ^ 1), 421)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&t_full[j % NK], TILE);
+#pragma unroll
+          for (int d = 0; d < SLABS; ++d) tma_load_4d(k_ring + (j % NK) * TILE + d * SLAB, &tmap_k, &t_full[j % NK], d * 64, 0, hk, where);
+        }
+        __syncwarp();
+        issued = 2 * j + 1;
+        if (!wait(&t_empty[NK + j % NV], (uint32_t)(((j / NV) & 1) ^ 1), 422)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&t_full[NK + j % NV], TILE);
+#pragma unroll
+          for (int d = 0; d < SLABS; ++d) tma_load_4d(v_ring + (j % NV) * TILE + d * SLAB, &tmap_v, &t_full[NK + j % NV], d * 64, 0, hk, where);
+        }
+        __syncwarp();
+        issued = 2 * j + 2;
+      }
+    }
+  } else if (warp == 9) {
+    bool ok = n_blocks == 0 || wait(q_full, 0, 423);
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    // S_t(j) = Q_t K(j)^T.  A page's keys are waited for by whichever tile comes first.
+    auto issue_qk = [&](int t, int j, bool wait_k) -> bool {
+      const int slot = j % NK;
+      if (wait_k && !wait(&t_full[slot], (uint32_t)((j / NK) & 1), 424)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t qdesc = make_smem_desc_sw128(smem_u32(q_smem + t * TILE), 16, 1024), kdesc = make_smem_desc_sw128(smem_u32(k_ring + slot * TILE), 16, 1024);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4;
+          umma_ss(tmem_base + (uint32_t)(t * 128), qdesc + off, kdesc + off, IDESC_QK, k != 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[t]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_pv = [&](int t, int j, bool wait_v) -> bool {
+      const int slot = j % NV;
+      if (wait_v && !wait(&t_full[NK + slot], (uint32_t)((j / NV) & 1), 426)) return false;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!wait(&p_ready[2 * t + half], (uint32_t)(j & 1), 425)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vdesc = make_smem_desc_sw128(smem_u32(v_ring + slot * TILE), SLAB, 1024);
+#pragma unroll
+          for (int k = 4 * half; k < 4 * half + 4; ++k)
+            umma_ts(tmem_base + (uint32_t)(256 + t * D), tmem_base + (uint32_t)(t * 128 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV, (j | k) != 0 ? 1u : 0u);
+          if (half == 1) umma_commit(&o_done[t]);
+        }
+        __syncwarp();
+      }
+      return true;
+    };
+    if (ok && n_blocks > 0) {
+      if (nblk[0] > 0) ok = issue_qk(0, 0, true);
+      if (ok && nblk[1] > 0) ok = issue_qk(1, 0, nblk[0] == 0);
+      if (ok) commit(&t_empty[0]);
+    }
+    for (int j = 0; ok && j < n_blocks; ++j) {
+      const bool a_now = j < nblk[0], b_now = j < nblk[1], a_next = j + 1 < nblk[0], b_next = j + 1 < nblk[1];
+      if (a_now) ok = issue_pv(0, j, true);
+      if (ok && a_next) ok = issue_qk(0, j + 1, true);
+      if (ok && b_now) ok = issue_pv(1, j, !a_now);
+      if (ok) commit(&t_empty[NK + j % NV]);
+      if (ok && b_next) ok = issue_qk(1, j + 1, !a_next);
+      if (ok && (a_next || b_next)) commit(&t_empty[(j + 1) % NK]);
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int t = warp >> 2, q = warp & 3, row = q * 32 + lane, nb = t ? nblk[1] : nblk[0], first = t ? tok0[1] : tok0[0];
+    const int i = first + row / group;            // this row's token; rows behind the tile's tokens see nothing
+    const bool real = row < per_tile * group && i < s.n;
+    const int last = real ? hidden + i : -1;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)(t * 128), o_addr = lane_addr + (uint32_t)(256 + t * D);
+    float m_used = -1e30f, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nb; ++j) {
+      ok = mbar_wait(&s_full[t], (uint32_t)(j & 1), abort_flag, p.err, 427);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const int kv0 = (j0 + j) * 128;
+      uint32_t r[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r + c * 32);
+      tmem_wait_ld();
+      if (kv0 + 127 > hidden + first) {           // some row does not see all of these keys
+        const int lim = last - kv0;
+#pragma unroll
+        for (int e = 0; e < 128; ++e)
+          if (e > lim) r[e] = __float_as_uint(-1e30f);
+      }
+      float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f;
+#pragma unroll
+      for (int e = 0; e < 128; e += 8) {
+        mx0 = pa_max3(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+        mx1 = pa_max3(mx1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+        mx2 = pa_max3(mx2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
+        mx3 = pa_max3(mx3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
+      }
+      const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * p.scale_log2;
+      float alpha = 1.f;
+      bool rescale = false;
+      if (j == 0) {
+        m_used = m_blk;
+      } else if (m_blk - m_used > 8.0f) {
+        alpha = pa_exp2(m_used - m_blk);
+        m_used = m_blk;
+        rescale = true;
+      }
+      if (__any_sync(0xffffffffu, rescale)) {
+        ok = mbar_wait(&o_done[t], (uint32_t)((j - 1) & 1), abort_flag, p.err, 428);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {        // narrow pieces: the 128 scores stay in registers meanwhile
+          uint32_t orr[16];
+          tmem_ld_32x16(o_addr + c * 16, orr);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * alpha);
+          tmem_st_32x16(o_addr + c * 16, orr);
+        }
+        l *= alpha;
+      }
+      if (kv0 + 128 > s.ctx && (t == 0 || j >= nblk[0])) {
+        // Behind the last key the page may hold anything, and 0 x NaN is none: those values become zeros, by the tile whose
+        // product comes first.
+        ok = mbar_wait(&t_full[NK + j % NV], (uint32_t)((j / NV) & 1), abort_flag, p.err, 429);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        if (kv0 + row >= s.ctx) {
+#pragma unroll
+          for (int d = 0; d < SLABS * 8; ++d) *reinterpret_cast<uint4*>(v_ring + (j % NV) * TILE + (d / 8) * SLAB + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_proxy();
+      }
+      // P = 2^(s c - m) as packed bf16 over the first 64 columns of S, handed over in two halves of 64 keys.  (Probabilities meet
+      // the values as bf16, the type of the tensor cores' other operand; their sum stays in fp32.)
+      float sum0 = 0.f, sum1 = 0.f;
+      const float neg_m = -m_used;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int e = 32 * half; e < 32 * half + 32; ++e) {
+          float x0, x1;
+          pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), p.scale_log2, neg_m);
+          const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
+          pa_add2(sum0, sum1, e0, e1);
+          r[e] = pack_bf16(e0, e1);
+        }
+        tmem_st_32x32(s_addr + half * 32, r + half * 32);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[2 * t + half]);
+      }
+      l += sum0 + sum1;
+    }
+    if (ok && nb > 0) {
+      ok = mbar_wait(&o_done[t], (uint32_t)((nb - 1) & 1), abort_flag, p.err, 430);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      tc_fence_after();
+      const bool sees = nb > 0 && last >= j0 * 128;      // a row that sees none of these keys has summed masked ones
+      const int h = hk * group + row % group;
+      const bool direct = plan.parts == 1;
+      const int64_t at = (((int64_t)plan.place + (int64_t)plan.item * plan.parts + plan.part) * p.Hkv + hk) * PT_ROWS + t * 128 + row;
+      if (real && !direct) out.part_ml[at] = sees ? make_float2(m_used, l) : make_float2(-1e30f, 0.f);
+      const float inv_l = sees ? 1.0f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t orr[32];
+        __syncwarp();
+        if (nb > 0) {
+          tmem_ld_32x32(o_addr + c * 32, orr);
+          tmem_wait_ld();
+        }
+        if (real && direct) {
+          uint4* to = reinterpret_cast<uint4*>(p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)h * p.so_h + c * 32);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (sees) {
+              uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) vv[e] = pack_bf16(__uint_as_float(orr[g * 8 + 2 * e]) * inv_l, __uint_as_float(orr[g * 8 + 2 * e + 1]) * inv_l);
+            }
+            to[g] = v;
+          }
+        } else if (real && sees) {
+          float4* to = reinterpret_cast<float4*>(out.part_o + at * D + c * 32);
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            to[g] = make_float4(__uint_as_float(orr[4 * g]), __uint_as_float(orr[4 * g + 1]), __uint_as_float(orr[4 * g + 2]), __uint_as_float(orr[4 * g + 3]));
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && warp == 8) {      // copies still on their way land before the block ends
+    if (n_blocks > 0) mbar_wait(q_full, 0, abort_flag + 1, p.err, 431);
+    for (int k = max(0, issued - 4); k < issued; ++k) {
+      const int j = k / 2, slot = k % 2 ? NK + j % NV : j % NK;
+      mbar_wait(&t_full[slot], (uint32_t)((j / 2) & 1), abort_flag + 1, p.err, 431);
+    }
+  }
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// Joins the parts of items that were cut: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A warp per token and head.  TILES: the
+// items of the kernel above, else one item a sequence, with `part_rows` rows.
+template <int D, bool TILES>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p, const PagedSplit in, int part_rows) {
   constexpr int W = D / 32;
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, b = blockIdx.z, h = blockIdx.y, group = p.Hq / p.Hkv, i = blockIdx.x * 8 + (threadIdx.x >> 5);
   const PagedSeq s = paged_seq(p, b);
-  if (i >= s.n || s.n * group > part_rows) return;
+  if (i >= s.n || (s.n * group > PA_FEW_ROWS) != TILES) return;
   const int2 plan = in.plan[b];
   if (plan.y <= 1) return;
-  const int hk = h / group, r = i * group + h % group;
-  auto place = [&](int k) { return ((int64_t)(plan.x + k) * p.Hkv + hk) * part_rows + r; };
+  const int hk = h / group, per_tile = 128 / group;
+  const int items = (s.n + 2 * per_tile - 1) / (2 * per_tile);
+  const int64_t first = TILES ? plan.x + (int64_t)(items - 1 - i / (2 * per_tile)) * plan.y : plan.x;
+  const int r = TILES ? i / per_tile % 2 * 128 + i % per_tile * group + h % group : i * group + h % group;
+  auto place = [&](int k) { return ((first + k) * p.Hkv + hk) * part_rows + r; };
   float M = -1e30f;
   for (int k = lane; k < plan.y; k += 32) M = fmaxf(M, in.part_ml[place(k)].x);
   M = warp_max(M);
@@ -485,7 +807,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   for (int k = 0; k < plan.y; ++k) {
     const int64_t at = place(k);
     const float2 x = in.part_ml[at];
-    const float w = x.y == 0.f ? 0.f : pa_exp2(x.x - M);
+    if (x.y == 0.f) continue;            // nothing was seen there, and nothing written
+    const float w = pa_exp2(x.x - M);
     L += w * x.y;
     const float* o = in.part_o + at * D + lane * W;
 #pragma unroll
@@ -497,6 +820,47 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   for (int e = 0; e < W; e += 2) *reinterpret_cast<__nv_bfloat162*>(o + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
 }
 
+// Blocks of a head that run at a time, and room for the sums of cut items.
+static int paged_split(const PagedParams& p, int ctas, int rows, PagedSplit* out) {
+  out->slots = ctas / p.Hkv;
+  if (out->slots < 1) out->slots = 1;
+  const uint64_t places = 2 * (uint64_t)out->slots * p.Hkv * rows;
+  void* scratch;
+  KD_TRY(get_workspace(places * (p.D * 4 + 8) + (uint64_t)p.B * 8, &scratch));
+  out->part_o = static_cast<float*>(scratch);
+  out->part_ml = reinterpret_cast<float2*>(out->part_o + places * p.D);
+  out->plan = reinterpret_cast<int2*>(out->part_ml + places);
+  return KD_OK;
+}
+
+// [token][head][D] with a box of the query heads of `tokens` tokens on one KV head, 64 channels wide.
+static int make_tmap_heads(CUtensorMap* out, const PagedParams& p, int group, int tokens) {
+  const int64_t ext[4] = {1, p.T, p.Hq, p.D}, st[3] = {p.T * p.sq_t, p.sq_t, p.sq_h};
+  return make_tmap_bhsd(out, p.q, ext, st, group, tokens);
+}
+
+template <int D>
+static int launch_tiles(const kd_tensor* k_pool, const kd_tensor* v_pool, const PagedParams& p) {
+  constexpr int SMEM = 6 * 128 * D * 2 + 1024 + 256;
+  static bool configured[64] = {false};   // per device: kd_shutdown + kd_init may move the library to another GPU
+  if (!configured[ctx().device & 63]) {
+    KD_CUDA_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    configured[ctx().device & 63] = true;
+  }
+  const int group = p.Hq / p.Hkv, per_tile = 128 / group;
+  CUtensorMap tq, tk, tv;
+  KD_TRY(make_tmap_heads(&tq, p, group, per_tile));
+  KD_TRY(make_tmap_bhsd(&tk, p.k, k_pool->shape, k_pool->strides, 128));
+  KD_TRY(make_tmap_bhsd(&tv, p.v, v_pool->shape, v_pool->strides, 128));
+  PagedSplit out{};
+  KD_TRY(paged_split(p, ctx().sm_count, PT_ROWS, &out));
+  const int64_t blocks = out.slots + (int64_t)p.T / (2 * per_tile) + p.B;     // items of all sequences, and one more for every cut
+  KD_CUDA_CHECK(launch_ex(paged_tiles_kernel<D>, dim3((unsigned)blocks, p.Hkv), dim3(PT_THREADS), (size_t)SMEM, tq, tk, tv, p, out));
+  KD_TRY(after_launch("paged_tiles_kernel"));
+  KD_CUDA_CHECK(launch_ex(paged_join_kernel<D, true>, dim3((p.max_query + 7) / 8, p.Hq, p.B), dim3(256), 0, p, out, PT_ROWS));
+  return after_launch("paged_join_kernel");
+}
+
 template <int D, int MT, int RG>
 static int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p) {
   using S = FewShape<D, MT, RG>;
@@ -506,18 +870,11 @@ static int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const PagedP
     configured[ctx().device & 63] = true;
   }
   PagedSplit out{};
-  out.slots = S::CTAS * ctx().sm_count / p.Hkv;
-  if (out.slots < 1) out.slots = 1;
-  const uint64_t places = 2 * (uint64_t)out.slots * p.Hkv * S::ROWS;
-  void* scratch;
-  KD_TRY(get_workspace(places * (D * 4 + 8) + (uint64_t)p.B * 8, &scratch));
-  out.part_o = static_cast<float*>(scratch);
-  out.part_ml = reinterpret_cast<float2*>(out.part_o + places * D);
-  out.plan = reinterpret_cast<int2*>(out.part_ml + places);
+  KD_TRY(paged_split(p, S::CTAS * ctx().sm_count, S::ROWS, &out));
   KD_CUDA_CHECK(launch_ex(paged_few_kernel<D, MT, RG>, dim3(out.slots + p.B, p.Hkv), dim3(S::THREADS), (size_t)S::SMEM, tk, tv, p, out));
   KD_TRY(after_launch("paged_few_kernel"));
   const int most = p.max_query * (p.Hq / p.Hkv) < S::ROWS ? p.max_query : S::ROWS / (p.Hq / p.Hkv);
-  KD_CUDA_CHECK(launch_ex(paged_join_kernel<D>, dim3((most + 7) / 8, p.Hq, p.B), dim3(256), 0, p, out, S::ROWS));
+  KD_CUDA_CHECK(launch_ex(paged_join_kernel<D, false>, dim3((most + 7) / 8, p.Hq, p.B), dim3(256), 0, p, out, S::ROWS));
   return after_launch("paged_join_kernel");
 }
 template <int D>
@@ -586,8 +943,7 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = ctx().error_flag;
   if ((int64_t)p.max_query * (Hq / Hkv) > PA_FEW_ROWS) {
-    KD_CUDA_CHECK(launch_ex(paged_attention_kernel, dim3((p.max_query + 7) / 8, Hq, B), dim3(256), 0, p));
-    KD_TRY(after_launch("paged_attention_kernel"));
+    KD_TRY(D == 128 ? launch_tiles<128>(k_pool, v_pool, p) : launch_tiles<64>(k_pool, v_pool, p));
     if (!q_start) return KD_OK;
   }
   return D == 128 ? few_rows<128>(k_pool, v_pool, p) : few_rows<64>(k_pool, v_pool, p);
