@@ -14,6 +14,9 @@ layer collapsed into 7 (prefill) / 3 (decode, larger batches or long contexts) k
                          one persistent kernel: o_proj -> residual+rms_norm -> gate/up with SiLU*up
                          -> down -> residual+rms_norm -> the NEXT layer's QKV partials
                          (tensor parallel: the same steps as separate kernels, with all-reduces)
+  extend, per layer      as prefill, behind the tokens that are there: QKV GEMM -> q/k-norm+RoPE+cache write -> attention of the new
+                         tokens over the cache (paged: kd_attention_paged)
+  beams (paged cache)    a decode step of all beams -> kd_beam_select -> kd_kv_pages_fork, in the same graph
   The decode step reads the write position / context length from device memory, so one captured
   graph is replayed for every step.
 
@@ -32,9 +35,10 @@ import math
 
 import numpy as np
 
-from . import core, lib, parallel
+from . import core, lib, paged, parallel
 from .core import Tensor
 from .model_utils.qwen3 import Qwen3Config
+from .model_utils.sampling import beam_select
 
 
 def _r(t):
@@ -183,7 +187,7 @@ class DecoderEngine:
 
 class Qwen3Engine(DecoderEngine):
     def __init__(self, cfg: Qwen3Config, weights, max_batch: int, max_seq_len: int, tp_size: int = 1, tp_rank: int = 0,
-                 paged: bool = False, page_table: np.ndarray | None = None):
+                 paged: bool = False, page_table: np.ndarray | None = None, spare_pages: int = 0):
         """weights: HuggingFace-style names -> float32 arrays (rounded to bf16 on upload), or a
         RandomInit.  With tp_size > 1 a weight dictionary is this rank's tensor-parallel slice
         (parallel.shard_qwen3_weights; a RandomInit draws rank `tp_rank`'s slice itself), cfg
@@ -192,7 +196,8 @@ class Qwen3Engine(DecoderEngine):
         paged=True keeps the KV cache in pools of 128-position pages [pages,Hkv,128,D] per layer,
         addressed through a block table int32 [max_batch, ceil(max_seq_len / 128)] (`page_table`, by
         default a fixed shuffle of all pages): same cache semantics as the contiguous StaticKVCache
-        (packages/model-utils/src/kv-cache.ts:164-212), same tokens."""
+        (packages/model-utils/src/kv-cache.ts:164-212), same tokens.  spare_pages: pages of every pool beyond those, for
+        beams (generate_beams), which need two partly filled pages each beside the whole ones that they share."""
         self.cfg = cfg
         self.tp = int(tp_size)
         self._init_decoding(max_batch, max_seq_len)
@@ -238,7 +243,8 @@ class Qwen3Engine(DecoderEngine):
             page_table = np.ascontiguousarray(page_table, dtype=np.int32)
             if page_table.shape != (self.B, per_seq) or page_table.min() < 0 or len(np.unique(page_table)) != n_pages:
                 raise ValueError(f"page_table must hold {n_pages} distinct page indices in a [{self.B},{per_seq}] array")
-            n_pool = int(page_table.max()) + 1
+            n_pool = int(page_table.max()) + 1 + int(spare_pages)
+            self.page_table = page_table
             self.block_table = Tensor(page_table)
             # pools [pages,Hkv,128,D] per layer, zero-initialised like the contiguous cache
             self.k_cache = [core.zeros((n_pool, self.Hkv, 128, self.D), "bfloat16") for _ in range(self.L)]
@@ -249,6 +255,7 @@ class Qwen3Engine(DecoderEngine):
             self.k_cache = [core.zeros((self.B, self.Hkv, max_seq_len, self.D), "bfloat16") for _ in range(self.L)]
             self.v_cache = [core.zeros((self.B, self.Hkv, max_seq_len, self.D), "bfloat16") for _ in range(self.L)]
         self.scale = 1.0 / math.sqrt(self.D)
+        self.cur_B = 0
         self._prefill_bufs = {}
         self.use_early_kv = os.environ.get("KD_EARLY_KV", "1") != "0"
         # decode: run o_proj .. next layer's QKV as one persistent kernel per layer (kd_decode_layer_chain);
@@ -347,11 +354,33 @@ class Qwen3Engine(DecoderEngine):
             }}
         return self._prefill_bufs[key]
 
-    def prefill(self, ids, all_logits: bool = False):
+    def prefill(self, ids, all_logits: bool = False, portion: int | None = None):
         """ids: host int32 array [B,S] (uploaded here) or an int32 device Tensor [B,S].  Fills the KV
         cache for positions [0,S) and returns the greedy next token per sequence as a device int64
         Tensor [B] (plus fp32 logits for every position when all_logits is set, which is what the
-        unmodified model code computes)."""
+        unmodified model code computes).  portion: tokens of a sequence that are run at a time (default: all), which bounds
+        the memory of the activations."""
+        if portion is not None and portion < 1:
+            raise ValueError(f"portions of {portion} tokens")
+        if portion is not None and portion < ids.shape[1]:
+            if ids.shape[1] > self.max_seq_len:
+                raise ValueError(f"prefill of {ids.shape[0]}x{ids.shape[1]} exceeds the engine's {self.B}x{self.max_seq_len}")
+            host = ids.dataAsync() if isinstance(ids, Tensor) else np.asarray(ids)
+            parts = [(self.extend if a else self.prefill)(np.ascontiguousarray(host[:, a:a + portion]), all_logits) for a in range(0, host.shape[1], portion)]
+            return (parts[-1][0], core.cat([p[1] for p in parts], 1)) if all_logits else parts[-1]
+        return self._run_prompt(ids, 0, all_logits)
+
+    def extend(self, ids, all_logits: bool = False):
+        """The next tokens ids [B,S] of the running sequences, whose cache holds self.pos positions: the rest of a prompt, or what a user
+        says next (a token that decode_step has just returned is not in the cache yet and comes first).  Returns what prefill does.
+        Each new token attends to everything before it (kd_attention_paged with a paged cache)."""
+        if self.pos and ids.shape[0] != self.cur_B:
+            raise ValueError(f"{ids.shape[0]} token rows for {self.cur_B} running sequences")
+        if self.pos + ids.shape[1] > self.max_seq_len:
+            raise ValueError(f"Cache overflow: trying to write to position {self.pos}-{self.pos + ids.shape[1]}, but maxSeqLen is {self.max_seq_len}")
+        return self._run_prompt(ids, self.pos, all_logits)
+
+    def _run_prompt(self, ids, start: int, all_logits: bool):
         if isinstance(ids, Tensor):
             B, S = ids.shape
             ids_t = ids.view(B * S)
@@ -370,25 +399,45 @@ class Qwen3Engine(DecoderEngine):
         # 2560 wide, 9 layers: 1024 2.62, 2.49; 3 x 701 4.52, 4.46)
         lib.call("kd_set_pdl", 3 if self.use_pdl and self.tp == 1 and B * S <= 16384 else 0)
         try:
-            full = self._prefill_kernels(w, ids_t, B, S, all_logits)
+            full = self._prefill_kernels(w, ids_t, B, S, start, all_logits)
         finally:
             lib.call("kd_set_pdl", 0)
-        self.pos = S
+        self.pos = start + S
         self.cur_B = B
         return (w["tok"], full) if all_logits else w["tok"]
 
-    def _prefill_kernels(self, w: dict, ids_t: Tensor, B: int, S: int, all_logits: bool):
+    def _attend_behind(self, w: dict, lw: dict, li: int, table, ctx, start: int) -> None:
+        """One layer's QKV, cache write and attention for tokens that stand behind position `start` > 0."""
+        eps = ctypes.c_float(self.cfg.rmsNormEps)
+        self._linear(w["x"], lw["wqkv"], w["qkv"])
+        if self.paged:
+            lib.call("kd_qkv_norm_rope_cachewrite_paged", _r(w["qkv"]), _r(lw["q_norm"]), _r(lw["k_norm"]), eps, _r(w["cos"]), _r(w["sin"]), _r(self.k_cache[li]),
+                     _r(self.v_cache[li]), _r(table), None, start, _r(w["q"]))
+            T = w["q"].shape[0] * w["q"].shape[1]
+            q, o = w["q"].view(T, self.Hq, self.D), w["attn"].view(T, self.Hq, self.D)
+            lib.call("kd_attention_paged", _r(q), _r(self.k_cache[li]), _r(self.v_cache[li]), _r(table), _r(ctx), None, 0, ctypes.c_float(self.scale), _r(o))
+            q.dispose()
+            o.dispose()
+            return
+        kc, vc = (t.slice([slice(0, w["q"].shape[0]), slice(None), slice(None), slice(None)]) for t in (self.k_cache[li], self.v_cache[li]))
+        lib.call("kd_qkv_norm_rope_cachewrite", _r(w["qkv"]), _r(lw["q_norm"]), _r(lw["k_norm"]), eps, _r(w["cos"]), _r(w["sin"]), _r(kc), _r(vc), None, start, _r(w["q"]))
+        lib.call("kd_window_attention", _r(w["q"]), _r(kc), _r(vc), None, ctypes.c_float(self.scale), 0, None, start, _r(w["attn"]))
+        kc.dispose()
+        vc.dispose()
+
+    def _prefill_kernels(self, w: dict, ids_t: Tensor, B: int, S: int, start: int, all_logits: bool):
         c = self.cfg
         T = B * S
         core._kernel("index_select")(self.embed._handle, ids_t._handle, {"dim": 0}, w["emb"]._handle)
         core.copy_(w["h"], w["emb"])                       # bf16 embedding rows -> fp32 residual stream
-        lib.call("kd_rope_table", _r(self.inv_freq), None, 0, S, _r(w["cos"]), _r(w["sin"]))
+        lib.call("kd_rope_table", _r(self.inv_freq), None, start, S, _r(w["cos"]), _r(w["sin"]))
+        ctx = core.full((1,), start + S, "int32") if start and self.paged else None
         q_bhsd = w["q"].permute([0, 2, 1, 3])
         o_bhsd = w["attn"].permute([0, 2, 1, 3])
         attn2d = w["attn"].view(T, self.Hq * self.D)
         h, h1 = w["h"], w["h1"]
         table = self.block_table.slice([slice(0, B), slice(None)]) if self.paged else None
-        native = self.tp == 1 and self.D == 128 and not self.paged
+        native = self.tp == 1 and self.D == 128 and not self.paged and not start
         # layers 0, 1 to 3, and the rest: descriptors are gathered (2.5 us a layer) while the GPU is at the layers before
         for a, b in ((0, 1), (1, 4), (4, self.L)) if native else ():
             if a < min(b, self.L):
@@ -403,7 +452,9 @@ class Qwen3Engine(DecoderEngine):
                 vc = self.v_cache[li].slice([slice(0, B), slice(None), slice(None), slice(None)])
             if self.tp == 1 or li == 0:
                 self._norm(h, lw["in_norm"], w["x"])     # (tensor parallel: later layers get x from the fused add+norm)
-            if self.D == 128:
+            if start:
+                self._attend_behind(w, lw, li, table, ctx, start)
+            elif self.D == 128:
                 # QKV GEMM whose epilogue does q/k-norm + RoPE + the KV-cache write
                 lib.call("kd_qkv_linear_norm_rope_cachewrite", _r(w["x"]), _r(lw["wqkv"]), _r(lw["q_norm"]), _r(lw["k_norm"]),
                          ctypes.c_float(c.rmsNormEps), _r(w["cos"]), _r(w["sin"]), _r(kc), _r(vc), 0, _r(w["q"]))
@@ -411,10 +462,13 @@ class Qwen3Engine(DecoderEngine):
                 self._linear(w["x"], lw["wqkv"], w["qkv"])
                 lib.call("kd_qkv_norm_rope_cachewrite", _r(w["qkv"]), _r(lw["q_norm"]), _r(lw["k_norm"]),
                          ctypes.c_float(c.rmsNormEps), _r(w["cos"]), _r(w["sin"]), _r(kc), _r(vc), None, 0, _r(w["q"]))
-            kp, vp = kc.slice(f":, :, :{S}, :"), vc.slice(f":, :, :{S}, :")
-            lib.call("kd_flash_attention", _r(q_bhsd), _r(kp), _r(vp), _r(o_bhsd), ctypes.c_float(self.scale), 1)
-            if self.paged:
-                lib.call("kd_kv_pages_write", _r(kp), _r(vp), _r(self.k_cache[li]), _r(self.v_cache[li]), _r(table), 0)
+            if not start:
+                kp, vp = kc.slice(f":, :, :{S}, :"), vc.slice(f":, :, :{S}, :")
+                lib.call("kd_flash_attention", _r(q_bhsd), _r(kp), _r(vp), _r(o_bhsd), ctypes.c_float(self.scale), 1)
+                if self.paged:
+                    lib.call("kd_kv_pages_write", _r(kp), _r(vp), _r(self.k_cache[li]), _r(self.v_cache[li]), _r(table), 0)
+                kp.dispose()
+                vp.dispose()
             if self.tp == 1:
                 self._linear(attn2d, lw["wo"], h1, resid=h, epi=1)
                 self._norm(h1, lw["post_norm"], w["x"])
@@ -431,8 +485,8 @@ class Qwen3Engine(DecoderEngine):
                 self._allreduce(w["part"])
                 nxt = self.layers[li + 1]["in_norm"] if li + 1 < self.L else self.final_norm
                 self._norm(w["part"], nxt, w["x"], resid=h1, sum_out=h)
-            for t in (kc, vc, kp, vp):
-                t.dispose()
+            kc.dispose()
+            vc.dispose()
         # tied lm_head on the last position of every sequence (select commutes with the row-wise matmul)
         h3 = h.view(B, S, self.H)
         last = h3.select(1, S - 1)
@@ -451,7 +505,7 @@ class Qwen3Engine(DecoderEngine):
             full = core.empty((B, S, self.V), "float32")
             self._linear(xa, self.embed, full)
             xa.dispose()
-        for t in (q_bhsd, o_bhsd, attn2d, h3, last):
+        for t in (q_bhsd, o_bhsd, attn2d, h3, last, *([ctx] if ctx is not None else [])):
             t.dispose()
         if table is not None:
             table.dispose()
@@ -474,7 +528,7 @@ class Qwen3Engine(DecoderEngine):
             return s.value
         p2p = self.tp > 1 and self.use_p2p and parallel.peer_buffers_ready()
         d = {
-            "B": B, "graph": {}, "chain": self.use_chain,
+            "B": B, "graph": {}, "beams": None, "chain": self.use_chain,
             # (tensor parallel: fp32 partial sums of all sequences must fit one 2 MiB exchange slot)
             "fused": self.use_fused_layer and (self.tp == 1 or (p2p and B * self.H * 4 <= (2 << 20))),
             "p2p": p2p,
@@ -516,9 +570,23 @@ class Qwen3Engine(DecoderEngine):
             return None, 0
         return core.zeros((n.value // 4,), "int32"), keys.value
 
-    def _form(self, d: dict) -> str:
+    def _kernels_of(self, d: dict) -> str:
         # by the position and not by the room in the cache: most engines are built for far longer contexts than a request has
         return "step" if d["step"] is not None and self.pos <= d["step_keys"] else "layers"
+
+    def _form(self, d: dict):
+        form = self._kernels_of(d)
+        return form if d["beams"] is None else (form, *d["beams"]["key"])
+
+    def _warm_decode_step(self, d: dict) -> None:
+        """With beams: a selection that writes elsewhere sizes the scratch; the beams, their tables and pages stay as they are."""
+        beams, d["beams"] = d["beams"], None
+        try:
+            self._enqueue_decode_step(d)
+        finally:
+            d["beams"] = beams
+        if beams is not None:
+            beam_select(beams["logits"], beams["scores"], beams["key"][2])
 
     def _enqueue_decode_step(self, d: dict) -> None:
         """One decode step for d['ids'] at device position d['pos']; leaves the next ids in d['ids']."""
@@ -528,17 +596,19 @@ class Qwen3Engine(DecoderEngine):
         lib.call("kd_set_pdl", (2 if self.use_early_kv else 1) if self.use_pdl else 0)
         try:
             self._decode_step_kernels(d)
+            if d["beams"] is not None:
+                self._beam_step(d["beams"])
         finally:
             lib.call("kd_set_pdl", 0)
 
     def _decode_step_kernels(self, d: dict) -> None:
         c, B = self.cfg, d["B"]
         eps = ctypes.c_float(c.rmsNormEps)
-        if self._form(d) == "step":
+        if self._kernels_of(d) == "step":
             lib.call("kd_decode_step", self._layer_refs(0, self.L), self.L, _r(self.embed), _r(self.final_norm), _r(d["ids"]), _r(self.inv_freq), _r(d["pos"]),
                      _r(d["ctx"]), eps, ctypes.c_float(self.scale), _r(self.block_table), _r(d["step"]), _r(d["logits"]),
-                     _r(d["ids"]) if self.sampler is None else None)
-            if self.sampler is not None:
+                     _r(d["ids"]) if self.sampler is None and d["beams"] is None else None)
+            if self.sampler is not None and d["beams"] is None:
                 lg = d["logits"].view(B, self.V)
                 self._next_tokens(lg, d["uniforms"], d["ids"])
                 lg.dispose()
@@ -608,12 +678,102 @@ class Qwen3Engine(DecoderEngine):
             kc.dispose()
             vc.dispose()
         lib.call("kd_linear_bf16_skinny", _r(d["x"]), _r(self.embed), 0, _r(d["logits"]))
-        lg = d["logits"].view(B, self.V)
-        self._next_tokens(lg, d["uniforms"], d["ids"])
-        lg.dispose()
+        if d["beams"] is None:
+            lg = d["logits"].view(B, self.V)
+            self._next_tokens(lg, d["uniforms"], d["ids"])
+            lg.dispose()
         lib.call("kd_increment_i32", _r(d["pos"]), 1)
         lib.call("kd_increment_i32", _r(d["ctx"]), 1)
         for t in (q_bh1d, o_bh1d, attn2d):
             t.dispose()
         if table is not None:
             table.dispose()
+
+    # ------------------------------------------------------------------ beams
+    def _beam_state(self, d: dict, B: int, K: int, eos: int) -> dict:
+        R = B * K
+        return {"key": (B, K, eos), "scores": core.zeros((B, K), "float32"), "parents": core.zeros((B, K), "int32"), "ended": core.zeros((B, K), "float32"),
+                "spare": core.zeros((R,), "int32"), "logits": d["logits"].view(B, K, self.V), "tokens": d["ids"].view(B, K),
+                "table": self.block_table.slice([slice(0, R), slice(None)]), "length": d["pos"], "pools": paged.Pools([*self.k_cache, *self.v_cache])}
+
+    def _beam_step(self, b: dict) -> None:
+        """The beams' next tokens, and the cache that stands behind each."""
+        beam_select(b["logits"], b["scores"], b["key"][2], out=(b["scores"], b["parents"], b["tokens"], b["ended"]))
+        paged.fork_pages(b["pools"], b["parents"], b["table"], b["spare"], b["length"])
+
+    def _fresh_pages(self, b: dict, book: paged.PagePool, table: np.ndarray, column: int) -> None:
+        """Every beam gets a page of its own for the positions from 128 * column on.  What the beams no longer name is free."""
+        R = len(table)
+        spare = b["spare"].dataAsync()
+        table[:, :column] = b["table"].dataAsync()[:, :column]
+        book.keep(np.concatenate([table[:, :column].reshape(-1), spare]))
+        table[:, column] = book.take(R)
+        core._backend().upload(b["table"]._handle, table)
+
+    def generate_beams(self, ids, beams: int, steps: int, eos: int = -1, length_penalty: float = 1.0, use_graph: bool = True) -> list:
+        """Beam search behind prompts ids [B,S] (paged cache, B * beams <= max_batch): up to `steps` tokens.  Returns, per prompt, up to `beams`
+        hypotheses (tokens, score), best first; score is the sum of the tokens' log-probabilities divided by their number to the power
+        length_penalty.  One that ends with `eos` leaves its beam to others; a prompt is done when `beams` have ended and the best running one
+        scores no higher than the worst of them.  Beams share the pages that they have in common.  The cache is free afterwards."""
+        if not self.paged:
+            raise ValueError("beams need a paged cache (paged=True)")
+        if self.tp > 1:
+            raise ValueError("beams are not implemented for tensor parallelism")
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        (B, S), K, R = ids.shape, int(beams), ids.shape[0] * int(beams)
+        if not 1 <= K <= 32 or R > self.B or steps < 1 or S < 1:
+            raise ValueError(f"{B} prompts of {S} tokens with {K} beams and {steps} steps: 1 to 32 beams, at most {self.B} in all, and one step at least")
+        if S + steps > self.max_seq_len:
+            raise ValueError(f"Cache overflow: {S} + {steps} positions, but maxSeqLen is {self.max_seq_len}")
+        sampler, self.sampler = self.sampler, None
+        try:
+            return self._generate_beams(ids, B, S, K, R, steps, int(eos), float(length_penalty), use_graph)
+        finally:
+            self.sampler = sampler
+            core._backend().upload(self.block_table._handle, self.page_table)
+            if self._decode is not None:
+                self._decode["beams"] = None
+            self.pos = self.cur_B = 0
+
+    def _generate_beams(self, ids, B: int, S: int, K: int, R: int, steps: int, eos: int, power: float, use_graph: bool) -> list:
+        self.prefill(ids)
+        d = self._decode_state(R)
+        states = d.setdefault("beam_states", {})
+        b = states.get((B, K, eos)) or states.setdefault((B, K, eos), self._beam_state(d, B, K, eos))
+        # the prompt's pages stand in the first beam's row; the others take them over as children of it
+        book, held, whole = paged.PagePool(self.k_cache[0].shape[0]), -(-S // paged.PAGE), S // paged.PAGE
+        book.keep(self.page_table[:B, :held])
+        table = np.zeros((R, self.page_table.shape[1]), np.int32)
+        table[::K, :held] = self.page_table[:B, :held]
+        if whole < held:
+            table[np.arange(R) % K != 0, whole] = book.take(R - B)
+        core._backend().upload(b["spare"]._handle, book.take(R))
+        core._backend().upload(b["table"]._handle, table)
+        logits = b["logits"].select(1, 0)
+        core.copy_(logits, self._prefill_bufs[(B, S)]["logits"].view(B, self.V))
+        logits.dispose()
+        scores = np.full((B, K), -np.inf, np.float32)
+        scores[:, 0] = 0.0
+        core._backend().upload(b["scores"]._handle, scores)
+        self._place(d)
+        self._beam_step(b)
+        d["beams"], d["use_graph"] = b, use_graph
+        running, ended = [[[]] * K for _ in range(B)], [[] for _ in range(B)]
+
+        def worth(score: float, n: int) -> float:
+            return float(score) / n ** power
+
+        for step in range(1, steps + 1):
+            parents, tokens, scores, ends = (b[n].dataAsync() for n in ("parents", "tokens", "scores", "ended"))
+            for i in range(B):
+                for j in np.flatnonzero(np.isfinite(ends[i])):
+                    ended[i].append((running[i][j] + [eos], worth(ends[i, j], step)))
+                ended[i] = sorted(ended[i], key=lambda h: -h[1])[:K]
+                running[i] = [running[i][p] + [int(t)] for p, t in zip(parents[i], tokens[i])]
+            done = [len(e) == K and e[-1][1] >= worth(s[0], step) for e, s in zip(ended, scores)]
+            if step == steps or all(done):
+                break
+            if self.pos % paged.PAGE == 0:
+                self._fresh_pages(b, book, table, self.pos // paged.PAGE)
+            self.decode_step()
+        return [sorted(e + [(r, worth(s, len(r))) for r, s in zip(rs, ss) if np.isfinite(s)], key=lambda h: -h[1])[:K] for e, rs, ss in zip(ended, running, scores)]

@@ -38,8 +38,9 @@ def load_config(folder: str) -> dict:
         return json.load(f)
 
 
-def load_engine(folder: str, max_batch: int, max_seq_len: int, dtype: str = "bfloat16"):
-    """Engine with the weights of `folder` (config.json and model.safetensors, or an index of shards)."""
+def load_engine(folder: str, max_batch: int, max_seq_len: int, dtype: str = "bfloat16", **options):
+    """Engine with the weights of `folder` (config.json and model.safetensors, or an index of shards).  options: more arguments of the
+    engine's class."""
     config = load_config(folder)
     entry = lookup(config)
     if dtype not in entry.dtypes:
@@ -47,7 +48,7 @@ def load_engine(folder: str, max_batch: int, max_seq_len: int, dtype: str = "bfl
     index = os.path.join(folder, "model.safetensors.index.json")
     group = io.loadSafetensor(index if os.path.exists(index) else os.path.join(folder, "model.safetensors"))
     try:
-        return entry.engine(entry.config(config, dtype), io.SafetensorStateDict(group), max_batch, max_seq_len)
+        return entry.engine(entry.config(config, dtype), io.SafetensorStateDict(group), max_batch, max_seq_len, **options)
     finally:
         group.close()
 
@@ -60,9 +61,9 @@ def _qwen3_config(c: dict, dtype: str):
                        rmsNormEps=c.get("rms_norm_eps", 1e-6), ropeTheta=c.get("rope_theta", 1e6), dtype=dtype)
 
 
-def _qwen3_engine(cfg, weights, max_batch, max_seq_len):
+def _qwen3_engine(cfg, weights, max_batch, max_seq_len, **options):
     from .engine import Qwen3Engine
-    return Qwen3Engine(cfg, weights, max_batch, max_seq_len)
+    return Qwen3Engine(cfg, weights, max_batch, max_seq_len, **options)
 
 
 def _pedorax_config(c: dict, dtype: str):
@@ -75,9 +76,9 @@ def _vogozen_config(c: dict, dtype: str):
     return VogozenConfig.fromDict(c, dtype)
 
 
-def _hybrid_engine(cfg, weights, max_batch, max_seq_len):
+def _hybrid_engine(cfg, weights, max_batch, max_seq_len, **options):
     from .hybrid_engine import HybridEngine
-    return HybridEngine(cfg, weights, max_batch, max_seq_len)
+    return HybridEngine(cfg, weights, max_batch, max_seq_len, **options)
 
 
 register("Qwen3ForCausalLM", ModelEntry(_qwen3_config, _qwen3_engine, ("bfloat16",)))
