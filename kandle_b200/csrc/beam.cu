@@ -389,6 +389,14 @@ __global__ void __launch_bounds__(BM_THREADS, 4) beam_kernel(const BeamParams p)
   if (sh.last) beam_join(p, b, sh);
 }
 
+// After an error of another kernel in between (context.cu, check_device_flag).
+int beam_reset_counters() {
+  void* at = nullptr;
+  KD_CUDA_CHECK(cudaGetSymbolAddress(&at, g_beam_through));
+  KD_CUDA_CHECK(cudaMemsetAsync(at, 0, sizeof(unsigned) * BM_REQUESTS, ctx().stream));
+  return KD_OK;
+}
+
 }  // namespace kd
 
 using namespace kd;
