@@ -2,6 +2,22 @@
 //
 // Sequence b brings n_b new tokens (packed rows of q), whose keys and values are the last n_b of its ctx_b positions in the pages:
 // token i sees positions 0 .. ctx_b - n_b + i.
+//
+// Tiles.  A tile of 128 rows holds the query heads that share a KV head of 128 / group tokens, a token's heads side by side; a page is a
+// key tile, found through the block table.  S = Q K^T and O += P V run on tcgen05 with S, P (packed bf16) and O in tensor memory, in two
+// chains of which one computes while the other waits.  An item of work is
+//   a sequence of up to 128 rows: the chains take its even and odd pages, and their sums are added at the end (bound: HBM), or
+//   two neighbouring tiles of a longer one: a chain each, both on every page (bound: exponentials beside the tensor pipe).
+//
+// Division.  The pages of all items of all KV heads stand in one row, and each of as many persistent blocks as SMs takes an equal share of it, from
+// wherever it begins in one item to wherever it ends in another: long and short sequences, prompts and single tokens load every SM
+// alike.  An item that is cut leaves unnormalised sums that are joined, by the block that is through last where they are small (up to
+// 32 rows), else by a second kernel.
+//
+// Softmax.  A thread owns a row and loads its 128 scores at once; S is free from then on, so that the next Q K^T runs beside the exponentials
+// (with P over S it waited for P V, and a chain's step was the sum of both: 4331 cycles for two tiles and a page, of which the exponential unit
+// needs 2048 and the tensor pipe 2048).  With heads of 128 tensor memory holds one S for both chains, which they use in turn, two P and two O; with heads of 64
+// two of each.  Two threads a row (and 16 warps) were slower: they have to exchange the maximum.
 #include "common.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
@@ -21,7 +37,6 @@ struct PagedParams {
   __nv_bfloat16* o;
   int64_t sq_t, sq_h, so_t, so_h, sk[3], sv[3];   // pools: page, head, row
   float scale_log2;
-  int behind_tiles;            // the kernel before belongs to the same call, and has no part in what this one reads
   int* err;
 };
 
@@ -42,10 +57,10 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
   return s;
 }
 
-// ----------------------------------------------------------------------------- what both kernels share
-// A tile of 128 rows holds the query heads that share a KV head of 128 / group tokens, a token's heads side by side; a page is a key
-// tile.  S = Q K^T and O += P V run on tcgen05 with S, P (over S, as packed bf16) and O in tensor memory; a thread owns a row.
-constexpr int PA_ROWS = 128;
+constexpr int PA_ROWS = 128;            // rows of a tile
+constexpr int PA_SOFTMAX = 8;           // warps 0-7: chain warp / 4, rows 32 (warp % 4) and on
+constexpr int PA_THREADS = 384;
+constexpr int PA_CACHE = 64;            // sequences whose lengths are kept in shared memory
 
 __device__ __forceinline__ float pa_exp2(float x) {
   float y;
@@ -73,867 +88,689 @@ __device__ __forceinline__ void pa_add2(float& s0, float& s1, float a0, float a1
       : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
 }
 
-// One key tile of a thread's row, whose scores are complete: the running maximum m (of scores times scale_log2) and sum l, P for the MMA
-// warp in two halves of 64 keys.  lim >= 0: only keys 0 .. lim of the tile are seen (masked; a row that sees none gets sums that its caller
-// drops).  The maximum is raised only when it grew by more than 2^8: the sum uses the same one, so nothing is lost.  before_p() comes
-// before P is handed over, o_ready() before O is touched; both return whether to go on, alike in a whole warp.
-template <int D, typename Ready, typename Before>
-__device__ __forceinline__ bool paged_softmax(uint32_t s_addr, uint32_t o_addr, bool masked, int lim, bool first, bool real, float scale_log2, float& m, float& l, uint64_t* p_ready,
-                                              Ready o_ready, Before before_p) {
-  tc_fence_after();
-  uint32_t r[128];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r + c * 32);
-  tmem_wait_ld();
-  if (masked) {
-#pragma unroll
-    for (int e = 0; e < 128; ++e)
-      if (e > lim) r[e] = __float_as_uint(-1e30f);
-  }
-  float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f;
-#pragma unroll
-  for (int e = 0; e < 128; e += 8) {
-    mx0 = pa_max3(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-    mx1 = pa_max3(mx1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
-    mx2 = pa_max3(mx2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
-    mx3 = pa_max3(mx3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
-  }
-  const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * scale_log2;
-  float alpha = 1.f;
-  bool rescale = false;
-  if (first || !real) {        // (nobody reads a padding row)
-    m = m_blk;
-  } else if (m_blk - m > 8.0f) {
-    alpha = pa_exp2(m - m_blk);
-    m = m_blk;
-    rescale = true;
-  }
-  if (__any_sync(0xffffffffu, rescale)) {
-    if (!o_ready()) return false;
-    tc_fence_after();
-#pragma unroll 1
-    for (int c = 0; c < D / 16; ++c) {            // narrow pieces: the 128 scores stay in registers meanwhile
-      uint32_t orr[16];
-      tmem_ld_32x16(o_addr + c * 16, orr);
-      tmem_wait_ld();
-#pragma unroll
-      for (int e = 0; e < 16; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * alpha);
-      tmem_st_32x16(o_addr + c * 16, orr);
-    }
-    l *= alpha;
-  }
-  if (!before_p()) return false;
-  // P = 2^(s c - m) as packed bf16 over the first 64 columns of S.  (Probabilities meet the values as bf16, the type of the tensor
-  // cores' other operand; their sum stays in fp32.)
-  float sum0 = 0.f, sum1 = 0.f;
-  const float neg_m = -m;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-#pragma unroll
-    for (int e = 32 * half; e < 32 * half + 32; ++e) {
-      float x0, x1;
-      pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), scale_log2, neg_m);
-      const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
-      pa_add2(sum0, sum1, e0, e1);
-      r[e] = pack_bf16(e0, e1);
-    }
-    tmem_st_32x32(s_addr + half * 32, r + half * 32);
-    tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(p_ready + half);
-  }
-  l += sum0 + sum1;
-  return true;
-}
-
-// Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them.  By the
-// four warps of a tile; `row` is the thread's key.
-template <int D>
-__device__ __forceinline__ void clear_values(uint8_t* tile, int row, int keys) {
-  if (row >= keys) {
-#pragma unroll
-    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<uint4*>(tile + (d / 8) * 16384 + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
-  }
-  fence_async_proxy();
-}
-
-// ----------------------------------------------------------------------------- up to 128 query rows: one pass over the keys at HBM speed
-// The key tiles of all sequences and KV heads stand in one row, and block x takes an equal share of it, from wherever it begins in one
-// sequence to wherever it ends in another; a sequence that is cut leaves unnormalised sums that are joined.  So long and short
-// sequences load every SM alike.
-//   warps 0-3   softmax of the even key tiles of the block's piece of a sequence, and its output
-//   warps 4-7   softmax of the odd ones: two chains of S, softmax and O, of which one computes while the other waits
-//   warp 8      divides the work; TMA: queries, then pages through a ring
-//   warp 9      tcgen05.mma
-//   warps 10-11 complete the third warpgroup, which hands registers to the softmax (72 against 216 a thread)
-// A warp whose rows are all padding only keeps step.  Bound: HBM; 128 exponentials a thread and tile are hidden behind the next pages.
-constexpr int PR_THREADS = 384, PR_CACHE = 40;      // (sequences whose lengths are kept in shared memory)
-struct RowSeq {
-  int row0, n, ctx, tiles;            // tiles: of keys, 1 for tokens without keys; 0 where another kernel has the sequence
+// ----------------------------------------------------------------------------- the division of the work
+// A sequence as an item of work sees it.  `units`: of all its items (0: no new tokens); a page of an item with two tiles counts twice, its two
+// softmaxes take twice as long.
+struct SeqWork {
+  int row0, n, ctx, units;
 };
-__device__ __forceinline__ RowSeq row_seq(const PagedParams& p, int b) {
-  const PagedSeq s = paged_seq(p, b);
-  const int rows = s.n * (p.Hq / p.Hkv);
-  return RowSeq{s.row0, s.n, s.ctx, rows == 0 || rows > PA_ROWS ? 0 : max(1, (s.ctx + 127) / 128)};
-}
-struct PagedSplit {
-  float* part_o;      // [place][rows][D] unnormalised sums
-  float2* part_ml;    // [place][rows] (running maximum in the log2 domain, sum)
-  int4* cut;          // the joining kernel's list: (sequence or first place, ..., parts)
-  int* cuts;          // its length
-  int slots;          // blocks of a head that run at a time
+struct ItemShape {
+  int group, tokens;                  // query heads on a KV head, tokens of a tile
+  __device__ __forceinline__ bool pair(int n) const { return n * group > PA_ROWS; }
+  __device__ __forceinline__ int items(int n) const { return pair(n) ? (n + 2 * tokens - 1) / (2 * tokens) : 1; }
+  // pages that an item's tokens see, and its units (one at least: tokens without keys get zero rows)
+  __device__ __forceinline__ int pages(const SeqWork& s, int item) const {
+    const int upto = pair(s.n) ? min(s.n, (item + 1) * 2 * tokens) : s.n;
+    return (max(0, s.ctx - s.n + upto) + 127) / 128;
+  }
+  __device__ __forceinline__ int units(const SeqWork& s, int item) const { return max(1, pages(s, item)) * (pair(s.n) ? 2 : 1); }
 };
-// Parts of a cut sequence that are through, by its first block; the last one sets it back.
-constexpr int PA_BLOCKS = 1024;
-static __device__ unsigned g_paged_through[PA_BLOCKS];
-// A piece of a sequence.
+__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, const ItemShape& shape, int b) {
+  const PagedSeq q = paged_seq(p, b);
+  SeqWork s{q.row0, q.n, q.ctx, 0};
+  if (q.n > 0)
+    for (int i = 0; i < shape.items(q.n); ++i) s.units += shape.units(s, i);
+  return s;
+}
+// A block's piece of an item: pages j0 .. j0 + nb - 1.
 struct Piece {
-  int b, hk, j0, nb;                  // key tiles j0 .. j0 + nb - 1
-  int parts, part, first;             // parts of the whole sequence, this one's number, the block of the first one
-  RowSeq s;
+  SeqWork s;
+  int b, hk, item, j0, nb;
+  int parts, part, first;             // parts of the whole item, this one's number, the block of the first one
+  bool pair;
+  // pages of the two chains
+  __device__ __forceinline__ void tiles(const ItemShape& shape, int (&n)[2]) const {
+    n[0] = (nb + 1) / 2;
+    n[1] = nb / 2;
+    if (!pair) return;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int token0 = (2 * item + t) * shape.tokens, keys = token0 >= s.n ? 0 : max(0, s.ctx - s.n + min(s.n, token0 + shape.tokens));
+      n[t] = min(max((keys + 127) / 128 - j0, 0), nb);
+    }
+  }
 };
-// Goes through the pieces of block x; the same in every warp.
+// Goes through the pieces of a block; the same in every warp.
 struct Walk {
-  int64_t u, end, per;                // place in the row of tiles
-  int b, hk, off;
-  __device__ __forceinline__ bool next(const PagedParams& p, const int4* cache, Piece& w) {
+  int64_t u, end, per;
+  int b, hk, item, off;
+  __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape& shape, const int4* cache, Piece& w) {
     if (u >= end) return false;
     for (;;) {
       if (b == p.B) { b = 0; ++hk; }
       if (hk == p.Hkv) return false;
-      if (b < PR_CACHE) { const int4 c = cache[b]; w.s = RowSeq{c.x, c.y, c.z, c.w}; }
-      else w.s = row_seq(p, b);
-      if (w.s.tiles) break;
+      if (b < PA_CACHE) { const int4 c = cache[b]; w.s = SeqWork{c.x, c.y, c.z, c.w}; }
+      else w.s = seq_work(p, shape, b);
+      if (w.s.units && item < shape.items(w.s.n)) break;
       ++b;
+      item = 0;
     }
-    const int64_t start = u - off, x = u / per;
-    w.b = b; w.hk = hk; w.j0 = off;
-    w.nb = (int)min((int64_t)(w.s.tiles - off), end - u);
+    w.pair = shape.pair(w.s.n);
+    const int all = shape.units(w.s, item), pages = shape.pages(w.s, item), weight = w.pair ? 2 : 1;
+    const int take = (int)min((int64_t)(all - off), end - u);
+    const int64_t start = u - off;
+    w.b = b; w.hk = hk; w.item = item;
+    w.j0 = min(off / weight, pages);
+    w.nb = min((off + take) / weight, pages) - w.j0;
     w.first = (int)(start / per);
-    w.parts = (int)((start + w.s.tiles - 1) / per) - w.first + 1;
-    w.part = (int)x - w.first;
-    u += w.nb;
-    ++b;
+    w.parts = (int)((start + all - 1) / per) - w.first + 1;
+    w.part = (int)(u / per) - w.first;
+    u += take;
     off = 0;
+    ++item;
     return true;
   }
 };
+// Block x's share, by one warp.
+__device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape& shape, int x, int blocks, int4* cache) {
+  const int lane = threadIdx.x & 31;
+  int64_t sum = 0;
+  for (int b = lane; b < p.B; b += 32) {
+    const SeqWork s = seq_work(p, shape, b);
+    if (b < PA_CACHE) cache[b] = make_int4(s.row0, s.n, s.ctx, s.units);
+    sum += s.units;
+  }
+  __syncwarp();
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int64_t all = sum * p.Hkv;
+  Walk w;
+  w.per = max((int64_t)1, (all + blocks - 1) / blocks);
+  w.u = min(all, x * w.per);
+  w.end = min(all, w.u + w.per);
+  w.hk = w.b = w.item = w.off = 0;
+  if (w.u >= w.end) return w;
+  w.hk = (int)(w.u / sum);
+  int64_t left = w.u - w.hk * sum;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b >= p.B ? 0 : b < PA_CACHE ? cache[b].w : seq_work(p, shape, b).units;
+    int64_t upto = n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, upto > left);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      w.b = b0 + who;
+      left -= __shfl_sync(0xffffffffu, upto - n, who);
+      break;
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  SeqWork s;
+  if (w.b < PA_CACHE) { const int4 c = cache[w.b]; s = SeqWork{c.x, c.y, c.z, c.w}; }
+  else s = seq_work(p, shape, w.b);
+  for (; left >= shape.units(s, w.item); ++w.item) left -= shape.units(s, w.item);
+  w.off = (int)left;
+  return w;
+}
 
-// Four channels of a row from all parts of a sequence: sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.  PIECES: part 0 ends block `first` (its
-// second place), the others begin the blocks behind it (their first places); else places first, first + 1, ...
-template <int D, bool PIECES>
-__device__ __forceinline__ void join_parts(const PagedParams& p, const PagedSplit& in, const RowSeq& s, int hk, int r, int c, int64_t first, int parts, int part_rows, int token = -1,
-                                           int head = 0) {
-  const int group = p.Hq / p.Hkv;
+// ----------------------------------------------------------------------------- sums of items that are cut
+// Block x leaves the end of an item that began before it at place 2 x, and the beginning of one that goes on behind it at 2 x + 1.
+struct PagedSplit {
+  float* part_o;      // [place][rows][D] unnormalised sums
+  float2* part_ml;    // [place][rows] (running maximum in the log2 domain, sum)
+  int4* cut;          // what began in block x and went on: (sequence, KV head, item, parts)
+};
+// Parts of a cut item that are through, by its first block; the last one sets it back.
+constexpr int PA_BLOCKS = 1024;
+static __device__ unsigned g_paged_through[PA_BLOCKS];
+
+// Four channels of a row from all parts of an item: sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
+template <int D>
+__device__ __forceinline__ void join_parts(const PagedSplit& in, int part_rows, int r, int c, int first, int parts, __nv_bfloat16* to) {
   float m = -1e30f, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int k = 0; k < parts; ++k) {
-    const int64_t at = (PIECES ? 2 * (first + k) + (k == 0 ? 1 : 0) : first + k) * part_rows + r;
+    const int64_t at = (int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * part_rows + r;
     const float2 x = __ldcg(in.part_ml + at);
     const float4 o = __ldcg(reinterpret_cast<const float4*>(in.part_o + at * D + c));
-    if (x.y == 0.f) continue;            // nothing was seen there
     const float now = fmaxf(m, x.x), f0 = pa_exp2(m - now), f1 = pa_exp2(x.x - now);
+    const bool some = x.y != 0.f;        // (else nothing was seen there, and nothing written)
     m = now;
-    l = l * f0 + x.y * f1;
-    acc.x = acc.x * f0 + o.x * f1; acc.y = acc.y * f0 + o.y * f1; acc.z = acc.z * f0 + o.z * f1; acc.w = acc.w * f0 + o.w * f1;
+    l = l * f0 + (some ? x.y * f1 : 0.f);
+    acc.x = acc.x * f0 + (some ? o.x * f1 : 0.f); acc.y = acc.y * f0 + (some ? o.y * f1 : 0.f);
+    acc.z = acc.z * f0 + (some ? o.z * f1 : 0.f); acc.w = acc.w * f0 + (some ? o.w * f1 : 0.f);
   }
-  if (token < 0) { token = r / group; head = r % group; }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + head) * p.so_h + c) =
-      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
-template <int D, int QROWS>
-struct RowShape {
-  static constexpr int TILE = 128 * D * 2, STAGES = 6 * 32768 / (2 * TILE);     // (keys and values)
-  static constexpr int Q_BYTES = QROWS * D * 2, QBUF = QROWS < 128 ? 2 : 1;
-  static constexpr int SMEM = 1024 + QBUF * Q_BYTES + STAGES * 2 * TILE + 256 + PR_CACHE * 16 + 128 + 1024;
+// ----------------------------------------------------------------------------- the kernel
+// FEW: no sequence has more than 32 rows; queries of two items and more pages fit, and a warp of its own writes the outputs.
+//   warps 0-7   softmax (and outputs)
+//   warp 8      FEW: outputs
+//   warp 9      division; TMA: queries, then pages through rings of keys and of values
+//   warps 10-11 tcgen05.mma: scores, products
+template <int D, bool FEW>
+struct PagedShape {
+  static constexpr int TILE = 128 * D * 2, RING = (FEW ? 3 : 2) * 32768 / TILE;      // slots for keys, and as many for values
+  static constexpr int QROWS = FEW ? 32 : PA_ROWS, Q_BYTES = QROWS * D * 2;
+  static constexpr int Q_AT = 0, RING_AT = 2 * Q_BYTES, BARS_AT = RING_AT + 2 * RING * TILE;
+  static constexpr int CACHE_AT = BARS_AT + 640, ML_AT = CACHE_AT + PA_CACHE * 16, BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
+  // tensor memory: scores, probabilities, sums
+  static constexpr int NS = D == 128 ? 1 : 2;
+  static constexpr uint32_t P_COL = 128 * NS, O_COL = P_COL + 128;
+  static_assert(O_COL + 2 * D == 512, "tensor memory has 512 columns");
+  static constexpr int SMEM = BYTES + 1024;
   static_assert(SMEM <= 227 * 1024, "tiles exceed shared memory");
 };
 
-template <int D, int QROWS>
-__global__ void __launch_bounds__(PR_THREADS, 1)
-paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                  const __grid_constant__ PagedParams p, const PagedSplit out) {
-  using S = RowShape<D, QROWS>;
-  constexpr int SLABS = D / 64, TILE = S::TILE, ST = S::STAGES, SLAB = 128 * 128, QSLAB = QROWS * 128, QBUF = S::QBUF;
+template <int D, bool FEW>
+__global__ void __launch_bounds__(PA_THREADS, 1)
+paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                       const __grid_constant__ PagedParams p, const PagedSplit out) {
+  using S = PagedShape<D, FEW>;
+  constexpr int SLABS = D / 64, TILE = S::TILE, RING = S::RING, SLAB = 128 * 128, QROWS = S::QROWS, QSLAB = QROWS * 128, Q_BYTES = S::Q_BYTES;
+  constexpr int NS = S::NS;
+  constexpr uint32_t P_COL = S::P_COL, O_COL = S::O_COL;
   constexpr uint32_t IDESC_QK = make_idesc_bf16(128, 128, 0, 0), IDESC_PV = make_idesc_bf16(128, D, 0, 1);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_smem = smem;                                   // (an MMA reads 128 rows: what follows stands in for the missing ones)
-  uint8_t* k_ring = q_smem + QBUF * S::Q_BYTES;
-  uint8_t* v_ring = k_ring + ST * TILE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_ring + ST * TILE);
-  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *o_done = bars + 10, *o_free = bars + 12;
-  uint64_t *k_full = bars + 13, *v_full = k_full + ST, *empty = v_full + ST;     // up to 6 each
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
-  int4* cache = reinterpret_cast<int4*>(bars + 32);
-  float2* ml = reinterpret_cast<float2*>(cache + PR_CACHE); // odd chain's (maximum, sum) of every row
-  Walk* walk_s = reinterpret_cast<Walk*>(ml + 128);
-  int* flags = reinterpret_cast<int*>(walk_s + 1);          // abort, and one that stays 0; whether this block joins
-  volatile int* abort_flag = flags;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.Hq / p.Hkv;
+  uint8_t *q_smem = smem + S::Q_AT, *ring = smem + S::RING_AT;      // (an MMA reads 128 rows: what follows stands in for missing ones)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS_AT);
+  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *o_done = bars + 10, *o_free = bars + 12, *few_done = bars + 13;
+  uint64_t *s_free = bars + 14, *y_bar = bars + 16;     // scores have been loaded [S]; sums of the two chains are there [quarter]
+  uint64_t *full = bars + 26, *empty = full + 2 * RING;      // up to 12 each
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);      // and behind it one that stays 0
+  int* joins = const_cast<int*>(abort_flag) + 2;                                  // items that this block joins at the end
+  Walk* walk_s = reinterpret_cast<Walk*>(bars + 52);
+  Piece* join_s = reinterpret_cast<Piece*>(walk_s + 1);                           // [2]
+  static_assert(52 * 8 + sizeof(Walk) + 2 * sizeof(Piece) <= 640, "barriers and what stands behind them");
+  int4* cache = reinterpret_cast<int4*>(smem + S::CACHE_AT);
+  float2* ml = reinterpret_cast<float2*>(smem + S::ML_AT);     // [piece & 1][chain][row] (maximum, sum)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const ItemShape shape{p.Hq / p.Hkv, QROWS / (p.Hq / p.Hkv)};
+  const int group = shape.group;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); }
-    for (int i = 0; i < 4; ++i) mbar_init(&p_ready[i], 4);
-    mbar_init(o_free, 4);
-    for (int i = 0; i < ST; ++i) { mbar_init(&k_full[i], 1); mbar_init(&v_full[i], 1); mbar_init(&empty[i], 1); }
-    flags[0] = flags[1] = 0;
+    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < 4; ++i) { mbar_init(&p_ready[i], 4); mbar_init(&y_bar[i], 2); }
+    mbar_init(o_free, FEW ? 1 : PA_SOFTMAX);
+    mbar_init(few_done, 2);
+    for (int i = 0; i < 2 * RING; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    abort_flag[0] = abort_flag[1] = 0;
+    *joins = 0;
     fence_mbar_init();
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
   }
-  if (warp == 9) {
+  if (warp == 10) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (!p.behind_tiles) pdl_wait();
-  if (warp == 8) {
-    // tiles of a head, and where this block begins
-    int64_t sum = 0;
-    for (int b = lane; b < p.B; b += 32) {
-      const RowSeq s = row_seq(p, b);
-      if (b < PR_CACHE) cache[b] = make_int4(s.row0, s.n, s.ctx, s.tiles);
-      sum += s.tiles;
-    }
-    __syncwarp();
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    Walk w;
-    const int64_t all = sum * p.Hkv;
-    w.per = max((int64_t)1, (all + gridDim.x - 1) / gridDim.x);
-    w.u = min(all, blockIdx.x * w.per);
-    w.end = min(all, w.u + w.per);
-    w.hk = w.b = w.off = 0;
-    if (w.u < w.end) {
-      w.hk = (int)(w.u / sum);
-      int64_t left = w.u - w.hk * sum;
-      for (int b0 = 0; b0 < p.B; b0 += 32) {
-        int n = 0;
-        if (b0 + lane < p.B) n = b0 + lane < PR_CACHE ? cache[b0 + lane].w : row_seq(p, b0 + lane).tiles;
-        int64_t upto = n;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, upto > left);
-        if (hit) {
-          const int who = __ffs(hit) - 1;
-          w.b = b0 + who;
-          w.off = (int)(left - __shfl_sync(0xffffffffu, upto - n, who));
-          break;
-        }
-        left -= __shfl_sync(0xffffffffu, upto, 31);
-      }
-    }
+  pdl_wait();
+  if (warp == 9) {
+    const Walk w = paged_walk(p, shape, blockIdx.x, gridDim.x, cache);
     if (lane == 0) *walk_s = w;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;      // S of chain t at 128 t, O at 256 + D t
+  const uint32_t tmem_base = *tmem_slot;      // S of chain t at 128 (t % NS), P at P_COL + 64 t, O at O_COL + D t
   pdl_trigger();                              // after the TMEM allocation (see common.cuh)
   Walk walk = *walk_s;
-  if (QROWS == PA_ROWS && threadIdx.x == 0) out.cut[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes what is cut, too)
+  if (!FEW && threadIdx.x == 0) out.cut[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes what is cut, too)
   Piece w;
-  const int q_tokens = QROWS / group;
-  int loaded = 0, q_loaded = 0;               // tiles (keys and values each) and queries asked for, by the copying warp
+  int issued[2] = {0, 0}, q_loaded = 0;       // pages' keys and values and items' queries asked for, by the copying warp
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code)); };
+  // where the outputs of a tile's row go
+  auto out_row = [&](const SeqWork& s, int hk, int token, int r) { return p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h; };
 
-  if (warp >= 8) {
+  if (warp >= PA_SOFTMAX) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp == 8) {
+  if (warp == 9) {
     bool ok = true;
-    for (; ok && walk.next(p, cache, w);) {
-      if (w.s.ctx == 0) continue;
-      const int qb = q_loaded % QBUF;
-      if (!wait(&q_empty[qb], (uint32_t)(((q_loaded / QBUF) & 1) ^ 1), 321)) break;
+    while (ok && walk.next(p, shape, cache, w)) {
+      if (w.nb == 0) continue;
+      int page = lane < w.nb ? p.table[w.b * p.table_row + w.j0 + lane] : 0;      // 32 entries of the table at a time
+      // queries: one item's two tiles, or FEW: two items' one tile
+      const int qb = FEW ? q_loaded & 1 : 0;
+      if (!wait(&q_empty[qb], (uint32_t)(((FEW ? q_loaded >> 1 : q_loaded) & 1) ^ 1), 321)) break;
+      const int tiles = w.pair ? 2 : 1, token0 = w.s.row0 + (w.pair ? w.item * 2 * shape.tokens : 0);
       if (elect_one()) {
-        mbar_arrive_expect_tx(&q_full[qb], SLABS * q_tokens * group * 128);
+        mbar_arrive_expect_tx(&q_full[qb], tiles * SLABS * shape.tokens * group * 128);
+        for (int t = 0; t < tiles; ++t)
 #pragma unroll
-        for (int d = 0; d < SLABS; ++d) tma_load_4d(q_smem + qb * S::Q_BYTES + d * QSLAB, &tmap_q, &q_full[qb], d * 64, w.hk * group, w.s.row0, 0);
+          for (int d = 0; d < SLABS; ++d)
+            tma_load_4d(q_smem + (qb + t) * Q_BYTES + d * QSLAB, &tmap_q, &q_full[qb], d * 64, w.hk * group, token0 + t * shape.tokens, 0);
       }
       __syncwarp();
       ++q_loaded;
-      int page = 0;
       for (int j = 0; j < w.nb; ++j) {
-        if (j % 32 == 0) {                    // 32 entries of the table at a time
-          page = j + lane < w.nb ? p.table[w.b * p.table_row + w.j0 + j + lane] : 0;
+        if (j % 32 == 0) {
+          if (j) page = j + lane < w.nb ? p.table[w.b * p.table_row + w.j0 + j + lane] : 0;
           if ((unsigned)page >= (unsigned)p.pages && atomicCAS(p.err, 0, 103) == 0) { p.err[1] = w.b; p.err[2] = page; }
         }
-        const int where = __shfl_sync(0xffffffffu, page, j % 32), slot = loaded % ST;
-        if (!(ok = wait(&empty[slot], (uint32_t)(((loaded / ST) & 1) ^ 1), 322))) break;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&k_full[slot], TILE);
+        const int where = __shfl_sync(0xffffffffu, page, j % 32);
 #pragma unroll
-          for (int d = 0; d < SLABS; ++d) tma_load_4d(k_ring + slot * TILE + d * SLAB, &tmap_k, &k_full[slot], d * 64, 0, w.hk, where);
-          mbar_arrive_expect_tx(&v_full[slot], TILE);
+        for (int v = 0; v < 2; ++v) {
+          const int slot = v * RING + issued[v] % RING;
+          if (!(ok = wait(&empty[slot], (uint32_t)(((issued[v] / RING) & 1) ^ 1), 322))) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&full[slot], TILE);
 #pragma unroll
-          for (int d = 0; d < SLABS; ++d) tma_load_4d(v_ring + slot * TILE + d * SLAB, &tmap_v, &v_full[slot], d * 64, 0, w.hk, where);
+            for (int d = 0; d < SLABS; ++d) tma_load_4d(ring + slot * TILE + d * SLAB, v ? &tmap_v : &tmap_k, &full[slot], d * 64, 0, w.hk, where);
+          }
+          __syncwarp();
+          ++issued[v];
         }
-        __syncwarp();
-        ++loaded;
+        if (!ok) break;
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 10) {
+    // Scores: S_t = Q_t K(g)^T in the order of pages and chains.  (A warp for the scores and one for the products: a wait takes some 200 cycles
+    // beside the operands that the tensor pipe reads from shared memory, and with ten waits and 32 MMAs for two tiles and a page one
+    // warp took 5700 cycles, more than the softmax.  One warp for each chain would not see every phase of the barriers that it waits for.)
     bool ok = true;
-    int done = 0, q_done = 0, pieces = 0, turn[2] = {0, 0};      // tiles, queries, pieces with keys, tiles of a chain
-    while (ok && walk.next(p, cache, w)) {
-      if (w.s.ctx == 0) continue;
-      const int qb = q_done % QBUF;
-      if (!(ok = wait(&q_full[qb], (uint32_t)((q_done / QBUF) & 1), 323))) break;
-      ++q_done;
-      // S(g) = Q K(g)^T, g-th tile of the piece
-      auto issue_qk = [&](int g) -> bool {
-        const int slot = (done + g) % ST, t = g & 1;
-        if (!wait(&k_full[slot], (uint32_t)(((done + g) / ST) & 1), 324)) return false;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t qdesc = make_smem_desc_sw128(smem_u32(q_smem + qb * S::Q_BYTES), 16, 1024), kdesc = make_smem_desc_sw128(smem_u32(k_ring + slot * TILE), 16, 1024);
+    int page = 0, q_done = 0, uses[2] = {0, 0};      // pages, items with keys, uses of an S
+    while (ok && walk.next(p, shape, cache, w)) {
+      if (w.nb == 0) continue;
+      const int qb = FEW ? q_done & 1 : 0;
+      const bool pair = !FEW && w.pair;
+      int n[2];
+      w.tiles(shape, n);
+      if (!(ok = wait(&q_full[qb], (uint32_t)((FEW ? q_done >> 1 : q_done) & 1), 324))) break;
+#pragma unroll 1
+      for (int g = 0; ok && g < w.nb; ++g, ++page) {
+        const int slot = page % RING;
+        if (!(ok = wait(&full[slot], (uint32_t)((page / RING) & 1), 325))) break;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_ss(tmem_base + (uint32_t)(t * 128), qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
-                    k != 0 ? 1u : 0u);
-          umma_commit(&s_full[t]);
-          if (g + 1 == w.nb) umma_commit(&q_empty[qb]);
-        }
-        __syncwarp();
-        return true;
-      };
-      for (int g = 0; ok && g < 2 && g < w.nb; ++g) ok = issue_qk(g);
-      // the sums of the piece before have been read
-      if (ok && pieces > 0) ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 325);
-      for (int g = 0; ok && g < w.nb; ++g) {
-        const int slot = (done + g) % ST, t = g & 1;
-        if (!(ok = wait(&v_full[slot], (uint32_t)(((done + g) / ST) & 1), 326))) break;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!(ok = wait(&p_ready[2 * t + half], (uint32_t)(turn[t] & 1), 327))) break;
+        for (int t = 0; t < 2; ++t) {
+          if (pair ? g >= n[t] : (g & 1) != t) continue;
+          constexpr int last_s = NS - 1;
+          const int sb = t & last_s;
+          if (uses[sb] > 0 && !(ok = wait(&s_free[sb], (uint32_t)((uses[sb] - 1) & 1), 340))) break;      // what was in it has been loaded
+          ++uses[sb];
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t vdesc = make_smem_desc_sw128(smem_u32(v_ring + slot * TILE), SLAB, 1024);
+            const uint64_t qdesc = make_smem_desc_sw128(smem_u32(q_smem + (qb + (pair ? t : 0)) * Q_BYTES), 16, 1024), kdesc = make_smem_desc_sw128(smem_u32(ring + slot * TILE), 16, 1024);
 #pragma unroll
-            for (int k = 4 * half; k < 4 * half + 4; ++k)
-              umma_ts(tmem_base + (uint32_t)(256 + t * D), tmem_base + (uint32_t)(t * 128 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV, g > 1 || k != 0 ? 1u : 0u);
-            if (half == 1) {
-              umma_commit(&empty[slot]);
-              umma_commit(&o_done[t]);
-            }
+            for (int k = 0; k < D / 16; ++k)
+              umma_ss(tmem_base + (uint32_t)(sb * 128), qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
+                      k != 0 ? 1u : 0u);
+            umma_commit(&s_full[t]);
           }
           __syncwarp();
         }
         if (!ok) break;
-        ++turn[t];
-        if (g + 2 < w.nb) ok = issue_qk(g + 2);
+        if (elect_one()) {
+          umma_commit(&empty[slot]);
+          if (g + 1 == w.nb) umma_commit(&q_empty[qb]);
+        }
+        __syncwarp();
       }
-      done += w.nb;
-      ++pieces;
+      ++q_done;
+    }
+  } else if (warp == 11) {
+    // Products: O_t += P_t V(g), in the same order.
+    bool ok = true;
+    int page = 0, q_done = 0, turn[2] = {0, 0};      // pages, items with keys, tiles of a chain
+    while (ok && walk.next(p, shape, cache, w)) {
+      if (w.nb == 0) continue;
+      const bool pair = !FEW && w.pair;
+      int n[2];
+      w.tiles(shape, n);
+      // the sums of the piece before have been read
+      if (q_done > 0 && !(ok = wait(o_free, (uint32_t)((q_done - 1) & 1), 328))) break;
+#pragma unroll 1
+      for (int g = 0; ok && g < w.nb; ++g, ++page) {
+        const int slot = RING + page % RING;
+        if (!(ok = wait(&full[slot], (uint32_t)((page / RING) & 1), 326))) break;
+#pragma unroll
+        for (int t = 0; ok && t < 2; ++t) {
+          if (pair ? g >= n[t] : (g & 1) != t) continue;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = wait(&p_ready[2 * t + half], (uint32_t)(turn[t] & 1), 327))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t vdesc = make_smem_desc_sw128(smem_u32(ring + slot * TILE), SLAB, 1024);
+#pragma unroll
+              for (int k = 4 * half; k < 4 * half + 4; ++k)
+                umma_ts(tmem_base + O_COL + (uint32_t)(t * D), tmem_base + P_COL + (uint32_t)(t * 64 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV,
+                        ((pair ? g : g >> 1) | k) != 0 ? 1u : 0u);
+              if (half == 1) umma_commit(&o_done[t]);
+            }
+            __syncwarp();
+          }
+          ++turn[t];
+        }
+        if (!ok) break;
+        if (elect_one()) umma_commit(&empty[slot]);
+        __syncwarp();
+      }
+      ++q_done;
+    }
+  } else if (FEW && warp == 8) {
+    // Outputs of pieces with up to 32 rows, while the chains go on.
+    int pieces = 0, turns[2] = {0, 0};
+    bool ok = true;
+    while (ok && walk.next(p, shape, cache, w)) {
+      const int rows = w.s.n * group;
+      const bool real = lane < rows, direct = w.parts == 1;
+      float f[2] = {0.f, 0.f}, M = -1e30f, L = 0.f;
+      const bool use[2] = {w.nb > 0, w.nb > 1};
+      if (w.nb > 0) {
+        if (!(ok = wait(few_done, (uint32_t)(pieces & 1), 337))) break;
+        const float2* now = ml + (pieces & 1) * 2 * PA_ROWS;
+        const float2 a = now[lane], b = now[PA_ROWS + lane];
+        M = fmaxf(a.x, b.x);
+        f[0] = a.y == 0.f ? 0.f : pa_exp2(a.x - M);
+        f[1] = b.y == 0.f ? 0.f : pa_exp2(b.x - M);
+        L = f[0] * a.y + f[1] * b.y;
+        if (direct) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          f[0] *= inv;
+          f[1] *= inv;
+        }
+        turns[0] += (w.nb + 1) / 2;
+        turns[1] += w.nb / 2;
+        if (!(ok = wait(&o_done[0], (uint32_t)((turns[0] - 1) & 1), 338))) break;
+        if (w.nb > 1 && !(ok = wait(&o_done[1], (uint32_t)((turns[1] - 1) & 1), 338))) break;
+        tc_fence_after();
+      }
+      __nv_bfloat16* to = real ? out_row(w.s, w.hk, lane / group, lane) : nullptr;
+      const int64_t at = (int64_t)(2 * blockIdx.x + (w.part == 0 ? 1 : 0)) * QROWS + lane;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        float o[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (!use[k]) continue;
+          uint32_t x[16];
+          __syncwarp();
+          tmem_ld_32x16(tmem_base + O_COL + k * D + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = f[k] == 0.f ? o[e] : fmaf(f[k], __uint_as_float(x[e]), o[e]);
+        }
+        if (real && direct) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]), pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(out.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      if (real && !direct) out.part_ml[at] = make_float2(M, L);
+      tc_fence_before();
+      __syncwarp();
+      if (w.nb > 0) {
+        ++pieces;
+        if (lane == 0) mbar_arrive(o_free);
+      }
+      if (!direct && lane == 0) {
+        // the part that is through last joins them all, at the end of its block (in the parts' order, whoever is last)
+        unsigned before;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(&g_paged_through[w.first]) : "memory");
+        if (before == (unsigned)w.parts - 1) {
+          g_paged_through[w.first] = 0;
+          join_s[*joins] = w;
+          ++*joins;
+        }
+      }
+      __syncwarp();
     }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int t = warp >> 2, q = warp & 3, row = q * 32 + lane, i = row / group;      // this row's token
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)(t * 128), o_addr = lane_addr + (uint32_t)(256 + t * D);
-    int done = 0, turn = 0, other = 0;      // tiles, this chain's, and for the even one those of the odd
+    const int t = warp >> 2, q = warp & 3, row = q * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)(t % NS * 128), p_addr = lane_addr + P_COL + (uint32_t)(t * 64), o_addr = lane_addr + O_COL + (uint32_t)(t * D);
+    const int row_token = row / group;
+    int done = 0, pieces = 0, turns[2] = {0, 0}, y_turn = 0;
     bool ok = true;
-    while (ok && walk.next(p, cache, w)) {
-      const int nb = w.s.ctx == 0 ? 0 : w.nb, hidden = w.s.ctx - w.s.n, rows = w.s.n * group;
-      const bool real = row < rows, active = q * 32 < rows;
-      const int last = real ? hidden + i : -1;                    // the last key that it sees
+    while (ok && walk.next(p, shape, cache, w)) {
+      const bool pair = !FEW && w.pair;
+      // this chain's tile
+      const int token0 = pair ? (2 * w.item + t) * shape.tokens : 0, tokens = min(shape.tokens, w.s.n - token0), rows = tokens * group;
+      const int hidden = w.s.ctx - w.s.n + token0;                  // keys 0 .. hidden + i are seen by the tile's token i
+      const bool active = q * 32 < rows, real = row < rows;
+      const int last = real ? hidden + row_token : -1;
+      int n[2];
+      w.tiles(shape, n);
+      const int mine = t ? n[1] : n[0];
+      int my_turn = t ? turns[1] : turns[0];
       float m = -1e30f, l = 0.f;
-      for (int g = t; g < nb; g += 2, ++turn) {
-        if (!(ok = wait(&s_full[t], (uint32_t)(turn & 1), 328))) break;
-        const int kv0 = (w.j0 + g) * 128, slot = (done + g) % ST;
-        auto before_p = [&] {
-          if (kv0 + 128 <= w.s.ctx) return true;
-          if (!wait(&v_full[slot], (uint32_t)(((done + g) / ST) & 1), 329)) return false;
-          clear_values<D>(v_ring + slot * TILE, row, w.s.ctx - kv0);
-          return true;
-        };
+      for (int i = 0; i < mine; ++i, ++my_turn) {
+        const int g = pair ? i : 2 * i + t, kv0 = (w.j0 + g) * 128;
+        if (!(ok = wait(&s_full[t], (uint32_t)(my_turn & 1), 329))) break;
+        tc_fence_after();
+        uint32_t r[128];
         if (active) {
-          ok = paged_softmax<D>(s_addr, o_addr, kv0 + 127 > hidden, last - kv0, g < 2, real, p.scale_log2, m, l, &p_ready[2 * t],
-                                [&] { return wait(&o_done[t], (uint32_t)((turn - 1) & 1), 330); }, before_p);
-          if (!ok) break;
-        } else {
-          if (!(ok = before_p())) break;
-          __syncwarp();
-          if (lane == 0) { mbar_arrive(&p_ready[2 * t]); mbar_arrive(&p_ready[2 * t + 1]); }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r + c * 32);
+          tmem_wait_ld();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t % NS]);
+        float alpha = 1.f;
+        bool rescale = false;
+        float neg_m = 0.f;
+        if (active) {
+          if (kv0 + 127 > hidden) {                                 // some row does not see all of these keys
+            const int lim = last - kv0;
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (e > lim) r[e] = __float_as_uint(-1e30f);
+          }
+          float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f;
+#pragma unroll
+          for (int e = 0; e < 128; e += 8) {
+            mx0 = pa_max3(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+            mx1 = pa_max3(mx1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+            mx2 = pa_max3(mx2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
+            mx3 = pa_max3(mx3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
+          }
+          const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * p.scale_log2;
+          // The maximum is raised only when it grew by more than 2^8: the sum uses the same one, so nothing is lost.
+          if (i == 0 || !real) {                                    // (nobody reads a padding row)
+            m = m_blk;
+          } else if (m_blk - m > 8.0f) {
+            alpha = pa_exp2(m - m_blk);
+            m = m_blk;
+            rescale = true;
+          }
+          neg_m = -m;
+        }
+        // P = 2^(s c - m) as packed bf16, handed over in two halves of 64 keys.  (Probabilities meet the values as bf16, the type of the
+        // tensor cores' other operand; their sum stays in fp32.)
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (active) {
+#pragma unroll
+            for (int e = 32 * half; e < 32 * half + 32; ++e) {
+              float x0, x1;
+              pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), p.scale_log2, neg_m);
+              const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
+              pa_add2(sum0, sum1, e0, e1);
+              r[e] = pack_bf16(e0, e1);
+            }
+          }
+          if (half == 0) {
+            // the product before has read P, and O is complete
+            if (my_turn > 0 && !(ok = wait(&o_done[t], (uint32_t)((my_turn - 1) & 1), 332))) break;
+            if (active && __any_sync(0xffffffffu, rescale)) {
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {                     // narrow pieces: the scores stay in registers meanwhile
+                uint32_t o[16];
+                tmem_ld_32x16(o_addr + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                tmem_st_32x16(o_addr + c, o);
+              }
+              l *= alpha;
+            }
+            if (kv0 + 128 > w.s.ctx && (!pair || t == 0 || i >= n[0])) {
+              // Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them (by
+              // the chain whose product comes first).
+              // (what stood in the slot before has been used, so that the parity is that of this page)
+              if (i == 0 && pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
+              const int slot = RING + (done + g) % RING;
+              if (!(ok = wait(&full[slot], (uint32_t)(((done + g) / RING) & 1), 330))) break;
+              if (kv0 + row >= w.s.ctx) {
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d) *reinterpret_cast<uint4*>(ring + slot * TILE + (d / 8) * SLAB + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_async_proxy();
+            }
+          }
+          if (active) {
+            tmem_st_32x32(p_addr + half * 32, r + half * 32);
+            tmem_wait_st();
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * t + half]);
+        }
+        if (!ok) break;
+        l += sum0 + sum1;
       }
       if (!ok) break;
-      done += nb;
-      other += nb / 2;
-      const int seen = min(last, (w.j0 + w.nb) * 128 - 1) - w.j0 * 128;        // the last key of the piece that the row sees
-      if (nb <= t || seen < t * 128) { m = -1e30f; l = 0.f; }                  // (a row that sees none of a chain's keys has summed masked ones)
-      if (nb > 1) {
-        if (t == 1) ml[row] = make_float2(m, l);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-      }
-      if (t == 1) continue;
-      // Both chains' sums.  (The odd one's next are behind the next product, which waits until these have been read.)
-      if (nb > 0 && !(ok = wait(&o_done[0], (uint32_t)((turn - 1) & 1), 331))) break;
-      if (nb > 1 && !(ok = wait(&o_done[1], (uint32_t)((other - 1) & 1), 331))) break;
-      tc_fence_after();
-      const float2 e = nb > 1 ? ml[row] : make_float2(-1e30f, 0.f);
-      const float M = fmaxf(m, e.x), wa = l == 0.f ? 0.f : pa_exp2(m - M), we = e.y == 0.f ? 0.f : pa_exp2(e.x - M), L = wa * l + we * e.y;
-      const bool direct = w.parts == 1;
-      const int64_t at = (int64_t)(2 * blockIdx.x + (w.part == 0 ? 1 : 0)) * QROWS + row;
-      const float f = !direct ? 1.f : L == 0.f ? 0.f : 1.f / L, fa = wa * f, fe = we * f;
-      if (active) {
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
-          uint32_t x[32];
+      done += w.nb;
+      turns[0] += n[0];
+      turns[1] += n[1];
+      // a row that sees none of the chain's keys has summed masked ones
+      const int first_key = (w.j0 + (pair ? 0 : t)) * 128;
+      if (mine == 0 || last < first_key) { m = -1e30f; l = 0.f; }
+      float2* now = ml + (pieces & 1) * 2 * PA_ROWS;
+      if constexpr (FEW) {
+        if (w.nb == 0) continue;
+        if (q == 0) {
+          // (the outputs of the piece before have been read: nobody is two pieces ahead)
+          if (pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
+          now[t * PA_ROWS + row] = make_float2(m, l);
           __syncwarp();
-          if (nb > 0) {
-            tmem_ld_32x32(lane_addr + 256 + c * 32, x);
-            tmem_wait_ld();
+          if (lane == 0) mbar_arrive(few_done);
+        }
+        ++pieces;
+        continue;
+      }
+      const bool direct = w.parts == 1;
+      const int place = 2 * blockIdx.x + (w.part == 0 ? 1 : 0);
+      if (threadIdx.x == 0 && !direct && w.part == 0) out.cut[blockIdx.x] = make_int4(w.b, w.hk, w.item, w.parts);
+      // the chains' shares of an output; where both worked on the same rows, each needs the other's statistics
+      float f[2] = {0.f, 0.f}, M = m, L = l;
+      if (w.nb > 0 && active) {
+        if (pair) {
+          f[t] = !direct ? 1.f : L == 0.f ? 0.f : 1.f / L;
+        } else {
+          now[t * PA_ROWS + row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&y_bar[q]);
+          if (!(ok = wait(&y_bar[q], (uint32_t)(y_turn & 1), 335))) break;
+          ++y_turn;
+          const float2 a = now[row], b = now[PA_ROWS + row];
+          M = fmaxf(a.x, b.x);
+          f[0] = a.y == 0.f ? 0.f : pa_exp2(a.x - M);
+          f[1] = b.y == 0.f ? 0.f : pa_exp2(b.x - M);
+          L = f[0] * a.y + f[1] * b.y;
+          if (direct) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            f[0] *= inv;
+            f[1] *= inv;
           }
+        }
+        if (n[0] > 0 && !(pair && t == 1) && !(ok = wait(&o_done[0], (uint32_t)((turns[0] - 1) & 1), 336))) break;
+        if (n[1] > 0 && !(pair && t == 0) && !(ok = wait(&o_done[1], (uint32_t)((turns[1] - 1) & 1), 336))) break;
+        tc_fence_after();
+      }
+      if (active) {
+        // this warp's channels: its own chain's, or half of both chains'
+        const int width = pair ? D : D / 2, c0 = pair ? 0 : t * width;
+        const bool use[2] = {w.nb > 0 && n[0] > 0 && !(pair && t == 1), w.nb > 0 && n[1] > 0 && !(pair && t == 0)};
+        __nv_bfloat16* to = real ? out_row(w.s, w.hk, token0 + row_token, row) : nullptr;
+        const int64_t at = (int64_t)place * (2 * PA_ROWS) + (pair ? t * PA_ROWS : 0) + row;
+#pragma unroll 1
+        for (int c = c0; c < c0 + width; c += 16) {
+          float o[16];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = fa == 0.f ? 0.f : fa * __uint_as_float(x[k]);
-          if (nb > 1) {
-            tmem_ld_32x32(lane_addr + 256 + D + c * 32, x);
+          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (!use[k]) continue;                                  // (alike in a whole warp)
+            uint32_t x[16];
+            __syncwarp();
+            tmem_ld_32x16(lane_addr + O_COL + k * D + c, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = fe == 0.f ? o[k] : fmaf(fe, __uint_as_float(x[k]), o[k]);
+            for (int e = 0; e < 16; ++e) o[e] = f[k] == 0.f ? o[e] : fmaf(f[k], __uint_as_float(x[e]), o[e]);
           }
           if (real && direct) {
-            uint4* to = reinterpret_cast<uint4*>(p.o + (int64_t)(w.s.row0 + i) * p.so_t + (int64_t)(w.hk * group + row % group) * p.so_h + c * 32);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              to[k] = make_uint4(pack_bf16(o[8 * k], o[8 * k + 1]), pack_bf16(o[8 * k + 2], o[8 * k + 3]), pack_bf16(o[8 * k + 4], o[8 * k + 5]), pack_bf16(o[8 * k + 6], o[8 * k + 7]));
+            for (int e = 0; e < 16; e += 8)
+              *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]), pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
           } else if (real) {
-            float4* to = reinterpret_cast<float4*>(out.part_o + at * D + c * 32);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(out.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        if (real && !direct) out.part_ml[at] = make_float2(M, L);
+        if (real && !direct && (pair || t == 0)) out.part_ml[at] = make_float2(M, L);
       }
+      if (w.nb == 0) continue;
+      // (nobody counts twice in a phase: the piece before is over)
+      if (pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
+      ++pieces;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0 && nb > 0) mbar_arrive(o_free);
-      if (direct) continue;
-      if constexpr (QROWS == PA_ROWS) {
-        // 64 KB a part and more: a second kernel joins them
-        if (threadIdx.x == 0 && w.part == 0) out.cut[blockIdx.x] = make_int4(w.b, w.hk, w.parts, 0);
-      } else {
-        // The part that is through last joins them all (in the parts' order, whoever is last).
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-        if (threadIdx.x == 0) {
-          unsigned before;
-          asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(&g_paged_through[w.first]) : "memory");
-          flags[2] = before == (unsigned)w.parts - 1;
-          if (flags[2]) g_paged_through[w.first] = 0;
-        }
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-        if (flags[2]) {
-          for (int n = threadIdx.x; n < rows * (D / 4); n += 128) {
-            const int r = n / (D / 4);
-            join_parts<D, true>(p, out, w.s, w.hk, r, n % (D / 4) * 4, w.first, w.parts, QROWS);
-          }
-        }
-      }
+      if (lane == 0) mbar_arrive(o_free);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag && warp == 8) {             // copies still on their way land before the block ends
-    if (q_loaded > 0) mbar_wait(&q_full[(q_loaded - 1) % QBUF], (uint32_t)(((q_loaded - 1) / QBUF) & 1), flags + 1, p.err, 332);
-    for (int k = max(0, loaded - ST); k < loaded; ++k) {
-      mbar_wait(&k_full[k % ST], (uint32_t)((k / ST) & 1), flags + 1, p.err, 332);
-      mbar_wait(&v_full[k % ST], (uint32_t)((k / ST) & 1), flags + 1, p.err, 332);
+  if (*abort_flag) {
+    if (warp == 9) {                         // copies still on their way land before the block ends
+      auto landed = [&](uint64_t* bar, int parity) { mbar_wait(bar, (uint32_t)(parity & 1), abort_flag + 1, p.err, 339); };
+      for (int i = max(0, q_loaded - (FEW ? 2 : 1)); i < q_loaded; ++i) landed(&q_full[FEW ? i & 1 : 0], FEW ? i >> 1 : i);
+      for (int v = 0; v < 2; ++v)
+        for (int i = max(0, issued[v] - RING); i < issued[v]; ++i) landed(&full[v * RING + i % RING], i / RING);
+    }
+  } else if (FEW) {
+    for (int i = 0; i < *joins; ++i) {
+      const Piece& j = join_s[i];
+      for (int n = threadIdx.x; n < j.s.n * group * (D / 4); n += PA_THREADS) {
+        const int r = n / (D / 4);
+        join_parts<D>(out, QROWS, r, n % (D / 4) * 4, j.first, j.parts, out_row(j.s, j.hk, r / group, r));
+      }
     }
   }
-  if (warp == 9) {
+  if (warp == 10) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
-  if (p.behind_tiles) pdl_wait();             // whoever waits for this kernel waits for the one before it
 }
 
-// Sequences with more than 32 rows that were cut.  Block x of the kernel above began with sequence cut[x] and did not end it; blocks of
-// 32 rows, four channels a thread.
+// Items of the kernel above that were cut and have more than 32 rows: block (x, y) has 32 rows of what began in block x and went on, four channels
+// a thread.
 template <int D>
-__global__ void __launch_bounds__(256) paged_rows_join_kernel(const __grid_constant__ PagedParams p, const PagedSplit in) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p, const PagedSplit in) {
   pdl_wait();
   pdl_trigger();
   const int4 c = in.cut[blockIdx.x];
-  if (c.z <= 1) return;
-  const RowSeq s = row_seq(p, c.x);
-  const int rows = s.n * (p.Hq / p.Hkv);
-  for (int n = threadIdx.x; n < 32 * (D / 4); n += 256) {
-    const int r = blockIdx.y * 32 + n / (D / 4);
-    if (r < rows) join_parts<D, true>(p, in, s, c.y, r, n % (D / 4) * 4, blockIdx.x, c.z, PA_ROWS);
-  }
-}
-
-// ----------------------------------------------------------------------------- many query rows: tcgen05
-// A block owns two tiles of 128 rows that share every key and passes over the pages of its part.
-//   warps 0-3   softmax and output of tile A, a row per thread      warps 4-7   the same for tile B
-//   warp 8      TMA: both query tiles, then the pages through two slots for keys and two for values
-//   warp 9      tcgen05.mma: QK_A(0) QK_B(0) | PV_A(j) QK_A(j+1) PV_B(j) QK_B(j+1) | ..., one tile's products beside the other's softmax
-//   warps 10-11 complete the third warpgroup, which hands registers to the softmax (72 against 216 a thread)
-// Bound: the softmax's issued instructions beside the tensor pipe.
-// How the work of every KV head is divided: per sequence `items` pairs of tiles with `len` key tiles each.  An item is cut into parts of at
-// most L key tiles where there are too few to fill the GPU, or where one is longer than a block's even share.
-struct PagedWork {
-  int items, len;
-};
-constexpr int PT_CACHE = 256;       // sequences whose work is kept in shared memory while L is looked for
-__device__ __forceinline__ PagedWork tile_work(const PagedParams& p, int b) {
-  const PagedSeq s = paged_seq(p, b);
-  const int group = p.Hq / p.Hkv, tokens = 2 * (PA_ROWS / group);
-  if (s.n * group <= PA_ROWS) return PagedWork{0, 0};
-  return PagedWork{(s.n + tokens - 1) / tokens, (s.ctx + 127) / 128};
-}
-__device__ __forceinline__ int parts_of(const PagedWork& w, int L) { return w.len <= L ? 1 : (w.len + L - 1) / L; }
-
-// What block x of a head does: part `part` of `parts` of item `item` of sequence b (-1: nothing).  Items that are cut have more than L tiles, so
-// there are at most `slots` of them and 2 x `slots` parts: `place` counts those before the item, `cut` the items, `cuts` all of them.
-struct PagedPlan {
-  int b, item, part, parts, place, cut, cuts;
-};
-// By one warp.  `slots`: blocks of a head that run at a time.
-__device__ __forceinline__ PagedPlan paged_plan(const PagedParams& p, int x, int slots, int least, int2* cache) {
-  const int lane = threadIdx.x & 31;
-  auto of = [&](int b) {
-    if (b < PT_CACHE) return PagedWork{cache[b].x, cache[b].y};
-    return tile_work(p, b);
-  };
-  int64_t sum = 0;
-  int longest = 0;
-  for (int b = lane; b < p.B; b += 32) {
-    const PagedWork w = tile_work(p, b);
-    if (b < PT_CACHE) cache[b] = make_int2(w.items, w.len);
-    sum += (int64_t)w.items * w.len;
-    longest = max(longest, w.len);
-  }
-  __syncwarp();
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  const int even = max(least, (int)((sum + slots - 1) / slots));
-  auto count = [&](int L) {
-    int n = 0;
-    for (int b = lane; b < p.B; b += 32) {
-      const PagedWork w = of(b);
-      n += w.items * parts_of(w, L);
-    }
-    return __reduce_add_sync(0xffffffffu, n);
-  };
-  // the smallest parts that run all at once; where that makes them a third longer than an even share, the even share
-  int L = even;
-  for (const int most = even + even / 3 + 1; L < longest && count(L) > slots;) {
-    L += max(1, L / 16);
-    if (L > most) {
-      L = even;
-      break;
-    }
-  }
-  PagedPlan plan{-1, 0, 0, 0, 0, 0, 0};
-  int before = 0, places = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const PagedWork w = b0 + lane < p.B ? of(b0 + lane) : PagedWork{0, 0};
-    const int parts = w.items ? parts_of(w, L) : 0, n = w.items * parts;
-    const int cut_parts = parts > 1 ? n : 0, cut_items = parts > 1 ? w.items : 0;
-    int upto = n, cut_upto = cut_parts, items_upto = cut_items;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o), u = __shfl_up_sync(0xffffffffu, cut_upto, o), y = __shfl_up_sync(0xffffffffu, items_upto, o);
-      if (lane >= o) { upto += v; cut_upto += u; items_upto += y; }
-    }
-    const int first = before + upto - n;
-    const unsigned hit = __ballot_sync(0xffffffffu, x >= first && x < first + n);
-    if (hit) {
-      const int who = __ffs(hit) - 1;
-      plan.b = b0 + who;
-      plan.parts = __shfl_sync(0xffffffffu, parts, who);
-      const int at = x - __shfl_sync(0xffffffffu, first, who);
-      plan.item = at / plan.parts;
-      plan.part = at % plan.parts;
-      plan.place = places + __shfl_sync(0xffffffffu, cut_upto - cut_parts, who) + plan.item * plan.parts;
-      plan.cut = plan.cuts + __shfl_sync(0xffffffffu, items_upto - cut_items, who) + plan.item;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-    places += __shfl_sync(0xffffffffu, cut_upto, 31);
-    plan.cuts += __shfl_sync(0xffffffffu, items_upto, 31);
-  }
-  return plan;
-}
-
-constexpr int PT_THREADS = 384, PT_ROWS = 256;
-
-template <int D>
-__global__ void __launch_bounds__(PT_THREADS, 1)
-paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                   const __grid_constant__ PagedParams p, const PagedSplit out) {
-  constexpr int SLABS = D / 64, NK = 2, NV = 2, TILE = 128 * D * 2, SLAB = 128 * 128;
-  constexpr uint32_t TMEM_COLS = 512;     // scores of tile t at 128 t, sums at 256 + D t
-  constexpr uint32_t IDESC_QK = make_idesc_bf16(128, 128, 0, 0), IDESC_PV = make_idesc_bf16(128, D, 0, 1);
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ int2 cache[PT_CACHE];
-  __shared__ PagedPlan plan_s;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_smem = smem;
-  uint8_t* k_ring = q_smem + 2 * TILE;
-  uint8_t* v_ring = k_ring + NK * TILE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_ring + NV * TILE);
-  uint64_t* q_full = bars;          // 1
-  uint64_t* t_full = bars + 1;      // 4: key slots, then value slots
-  uint64_t* t_empty = bars + 5;     // 4
-  uint64_t* s_full = bars + 9;      // 2
-  uint64_t* p_ready = bars + 11;    // 4: [tile][half of the keys]
-  uint64_t* o_done = bars + 15;     // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);     // and behind it one that stays 0
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y, group = p.Hq / p.Hkv, per_tile = 128 / group;
-
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int i = 0; i < NK + NV; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 1); }
-    for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&o_done[t], 1); }
-    for (int t = 0; t < 4; ++t) mbar_init(&p_ready[t], 4);
-    abort_flag[0] = abort_flag[1] = 0;
-    fence_mbar_init();
-    prefetch_tmap(&tmap_q);
-    prefetch_tmap(&tmap_k);
-    prefetch_tmap(&tmap_v);
-  }
-  pdl_wait();
-  if (warp == 8) {
-    const PagedPlan plan = paged_plan(p, blockIdx.x, out.slots, 2, cache);
-    if (lane == 0) {
-      plan_s = plan;
-      if (hk == 0 && blockIdx.x == 0) *out.cuts = plan.cuts;
-      if (hk == 0 && plan.b >= 0 && plan.part == 0 && plan.parts > 1) out.cut[plan.cut] = make_int4(plan.b, plan.item, plan.parts, plan.place);
-    }
-  }
-  __syncthreads();
-  const PagedPlan plan = plan_s;
-  if (plan.b < 0) return;
-  if (warp == 9) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  pdl_trigger();   // after the TMEM allocation (see common.cuh)
-
-  const PagedSeq s = paged_seq(p, plan.b);
-  const int hidden = s.ctx - s.n;                 // keys 0 .. hidden + i are seen by token i
-  // the last tokens, which see the most keys, begin first
-  const int items = (s.n + 2 * per_tile - 1) / (2 * per_tile), item = items - 1 - plan.item;
-  int tok0[2], nblk[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    tok0[t] = (2 * item + t) * per_tile;
-    nblk[t] = tok0[t] >= s.n ? 0 : (max(0, hidden + min(s.n, tok0[t] + per_tile)) + 127) / 128;
-  }
-  const int all = max(nblk[0], nblk[1]), j0 = (int)((int64_t)all * plan.part / plan.parts), n_blocks = (int)((int64_t)all * (plan.part + 1) / plan.parts) - j0;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) nblk[t] = min(max(nblk[t] - j0, 0), n_blocks);     // block numbers below count from j0
-
-  int issued = 0;                                 // pages' keys and values by the copying warp
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  // whole warps wait and an elected lane issues (see attention_prefill2.cu)
-  auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code)); };
-  if (warp == 8) {
-    if (n_blocks > 0) {
-      if (elect_one()) {
-        mbar_arrive_expect_tx(q_full, 2 * SLABS * per_tile * group * 128);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int d = 0; d < SLABS; ++d) tma_load_4d(q_smem + t * TILE + d * SLAB, &tmap_q, q_full, d * 64, hk * group, s.row0 + tok0[t], 0);
-      }
-      __syncwarp();
-      int page = 0;
-      for (int j = 0; j < n_blocks; ++j) {
-        if (j % 32 == 0) {       // 32 entries of the table at a time
-          page = j + lane < n_blocks ? p.table[plan.b * p.table_row + j0 + j + lane] : 0;
-          if ((unsigned)page >= (unsigned)p.pages && atomicCAS(p.err, 0, 103) == 0) { p.err[1] = plan.b; p.err[2] = page; }
-        }
-        const int where = __shfl_sync(0xffffffffu, page, j % 32);
-        if (!wait(&t_empty[j % NK], (uint32_t)(((j / NK) & 1) ^ 1), 421)) break;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&t_full[j % NK], TILE);
-#pragma unroll
-          for (int d = 0; d < SLABS; ++d) tma_load_4d(k_ring + (j % NK) * TILE + d * SLAB, &tmap_k, &t_full[j % NK], d * 64, 0, hk, where);
-        }
-        __syncwarp();
-        issued = 2 * j + 1;
-        if (!wait(&t_empty[NK + j % NV], (uint32_t)(((j / NV) & 1) ^ 1), 422)) break;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&t_full[NK + j % NV], TILE);
-#pragma unroll
-          for (int d = 0; d < SLABS; ++d) tma_load_4d(v_ring + (j % NV) * TILE + d * SLAB, &tmap_v, &t_full[NK + j % NV], d * 64, 0, hk, where);
-        }
-        __syncwarp();
-        issued = 2 * j + 2;
-      }
-    }
-  } else if (warp == 9) {
-    bool ok = n_blocks == 0 || wait(q_full, 0, 423);
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
-    };
-    // S_t(j) = Q_t K(j)^T.  A page's keys are waited for by whichever tile comes first.
-    auto issue_qk = [&](int t, int j, bool wait_k) -> bool {
-      const int slot = j % NK;
-      if (wait_k && !wait(&t_full[slot], (uint32_t)((j / NK) & 1), 424)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t qdesc = make_smem_desc_sw128(smem_u32(q_smem + t * TILE), 16, 1024), kdesc = make_smem_desc_sw128(smem_u32(k_ring + slot * TILE), 16, 1024);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4;
-          umma_ss(tmem_base + (uint32_t)(t * 128), qdesc + off, kdesc + off, IDESC_QK, k != 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[t]);
-      }
-      __syncwarp();
-      return true;
-    };
-    auto issue_pv = [&](int t, int j, bool wait_v) -> bool {
-      const int slot = j % NV;
-      if (wait_v && !wait(&t_full[NK + slot], (uint32_t)((j / NV) & 1), 426)) return false;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (!wait(&p_ready[2 * t + half], (uint32_t)(j & 1), 425)) return false;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t vdesc = make_smem_desc_sw128(smem_u32(v_ring + slot * TILE), SLAB, 1024);
-#pragma unroll
-          for (int k = 4 * half; k < 4 * half + 4; ++k)
-            umma_ts(tmem_base + (uint32_t)(256 + t * D), tmem_base + (uint32_t)(t * 128 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV, (j | k) != 0 ? 1u : 0u);
-          if (half == 1) umma_commit(&o_done[t]);
-        }
-        __syncwarp();
-      }
-      return true;
-    };
-    if (ok && n_blocks > 0) {
-      if (nblk[0] > 0) ok = issue_qk(0, 0, true);
-      if (ok && nblk[1] > 0) ok = issue_qk(1, 0, nblk[0] == 0);
-      if (ok) commit(&t_empty[0]);
-    }
-    for (int j = 0; ok && j < n_blocks; ++j) {
-      const bool a_now = j < nblk[0], b_now = j < nblk[1], a_next = j + 1 < nblk[0], b_next = j + 1 < nblk[1];
-      if (a_now) ok = issue_pv(0, j, true);
-      if (ok && a_next) ok = issue_qk(0, j + 1, true);
-      if (ok && b_now) ok = issue_pv(1, j, !a_now);
-      if (ok) commit(&t_empty[NK + j % NV]);
-      if (ok && b_next) ok = issue_qk(1, j + 1, !a_next);
-      if (ok && (a_next || b_next)) commit(&t_empty[(j + 1) % NK]);
-    }
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int t = warp >> 2, q = warp & 3, row = q * 32 + lane, nb = t ? nblk[1] : nblk[0], first = t ? tok0[1] : tok0[0];
-    const int i = first + row / group;            // this row's token; rows behind the tile's tokens see nothing
-    const bool real = row < per_tile * group && i < s.n;
-    const int last = real ? hidden + i : -1;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)(t * 128), o_addr = lane_addr + (uint32_t)(256 + t * D);
-    float m_used = -1e30f, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < nb; ++j) {
-      ok = mbar_wait(&s_full[t], (uint32_t)(j & 1), abort_flag, p.err, 427);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      const int kv0 = (j0 + j) * 128;
-      auto o_ready = [&] { return (bool)__all_sync(0xffffffffu, mbar_wait(&o_done[t], (uint32_t)((j - 1) & 1), abort_flag, p.err, 428)); };
-      auto before_p = [&] {
-        // (by the tile whose product comes first)
-        if (kv0 + 128 <= s.ctx || (t == 1 && j < nblk[0])) return true;
-        if (!__all_sync(0xffffffffu, mbar_wait(&t_full[NK + j % NV], (uint32_t)((j / NV) & 1), abort_flag, p.err, 429))) return false;
-        clear_values<D>(v_ring + (j % NV) * TILE, row, s.ctx - kv0);
-        return true;
-      };
-      if (!(ok = paged_softmax<D>(s_addr, o_addr, kv0 + 127 > hidden + first, last - kv0, j == 0, real, p.scale_log2, m_used, l, &p_ready[2 * t], o_ready, before_p))) break;
-    }
-    if (ok && nb > 0) {
-      ok = mbar_wait(&o_done[t], (uint32_t)((nb - 1) & 1), abort_flag, p.err, 430);
-      ok = __all_sync(0xffffffffu, ok);
-    }
-    if (ok) {
-      tc_fence_after();
-      const bool sees = nb > 0 && last >= j0 * 128;      // a row that sees none of these keys has summed masked ones
-      const int h = hk * group + row % group;
-      const bool direct = plan.parts == 1;
-      const int64_t at = ((int64_t)hk * 2 * out.slots + plan.place + plan.part) * PT_ROWS + t * 128 + row;
-      if (real && !direct) out.part_ml[at] = sees ? make_float2(m_used, l) : make_float2(-1e30f, 0.f);
-      const float inv_l = sees ? 1.0f / l : 0.f;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t orr[32];
-        __syncwarp();
-        if (nb > 0) {
-          tmem_ld_32x32(o_addr + c * 32, orr);
-          tmem_wait_ld();
-        }
-        if (real && direct) {
-          uint4* to = reinterpret_cast<uint4*>(p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)h * p.so_h + c * 32);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (sees) {
-              uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) vv[e] = pack_bf16(__uint_as_float(orr[g * 8 + 2 * e]) * inv_l, __uint_as_float(orr[g * 8 + 2 * e + 1]) * inv_l);
-            }
-            to[g] = v;
-          }
-        } else if (real && sees) {
-          float4* to = reinterpret_cast<float4*>(out.part_o + at * D + c * 32);
-#pragma unroll
-          for (int g = 0; g < 8; ++g)
-            to[g] = make_float4(__uint_as_float(orr[4 * g]), __uint_as_float(orr[4 * g + 1]), __uint_as_float(orr[4 * g + 2]), __uint_as_float(orr[4 * g + 3]));
-        }
-      }
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag && warp == 8) {      // copies still on their way land before the block ends
-    if (n_blocks > 0) mbar_wait(q_full, 0, abort_flag + 1, p.err, 431);
-    for (int k = max(0, issued - 4); k < issued; ++k) {
-      const int j = k / 2, slot = k % 2 ? NK + j % NV : j % NK;
-      mbar_wait(&t_full[slot], (uint32_t)((j / 2) & 1), abort_flag + 1, p.err, 431);
-    }
-  }
-  if (warp == 9) {
-    __syncwarp();
-    tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
-  }
-}
-
-// Items that were cut: block (x, y, z) has 32 rows of the x-th of head y, four channels a thread.
-template <int D>
-__global__ void __launch_bounds__(256) paged_tiles_join_kernel(const __grid_constant__ PagedParams p, const PagedSplit in) {
-  pdl_wait();
-  pdl_trigger();
-  if ((int)blockIdx.x >= *in.cuts) return;
-  const int4 c = in.cut[blockIdx.x];
+  if (c.w <= 1) return;
+  const ItemShape shape{p.Hq / p.Hkv, PA_ROWS / (p.Hq / p.Hkv)};
   const PagedSeq s = paged_seq(p, c.x);
-  const int group = p.Hq / p.Hkv, per_tile = PA_ROWS / group, items = (s.n + 2 * per_tile - 1) / (2 * per_tile);
+  const bool pair = shape.pair(s.n);
   for (int n = threadIdx.x; n < 32 * (D / 4); n += 256) {
-    const int r = blockIdx.z * 32 + n / (D / 4), i = (2 * (items - 1 - c.y) + r / PA_ROWS) * per_tile + r % PA_ROWS / group;
-    if (r % PA_ROWS < per_tile * group && i < s.n)
-      join_parts<D, false>(p, in, RowSeq{s.row0, s.n, s.ctx, 0}, blockIdx.y, r, n % (D / 4) * 4, (int64_t)blockIdx.y * 2 * in.slots + c.w, c.z, PT_ROWS, i, r % PA_ROWS % group);
+    const int r = blockIdx.y * 32 + n / (D / 4), i = (pair ? (2 * c.z + r / PA_ROWS) * shape.tokens : 0) + r % PA_ROWS / shape.group;
+    if (r % PA_ROWS >= shape.tokens * shape.group || i >= s.n || (!pair && r >= PA_ROWS)) continue;
+    join_parts<D>(in, 2 * PA_ROWS, r, n % (D / 4) * 4, blockIdx.x, c.w, p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)(c.y * shape.group + r % PA_ROWS % shape.group) * p.so_h);
   }
 }
 
-// As launch_ex, always with a programmatic dependency on the kernel before: for kernels that belong to the same call.
+// As launch_ex, always with a programmatic dependency on the kernel before: for a kernel that belongs to the same call.
 template <typename... KArgs, typename... Args>
 static cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
   const bool pdl = ctx().pdl;
@@ -943,82 +780,37 @@ static cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block
   return e;
 }
 
-// [token][head][D] with a box of the query heads of `tokens` tokens on one KV head, 64 channels wide.
-static int make_tmap_heads(CUtensorMap* out, const PagedParams& p, int tokens) {
-  const int64_t ext[4] = {1, p.T, p.Hq, p.D}, st[3] = {p.T * p.sq_t, p.sq_t, p.sq_h};
-  return make_tmap_bhsd(out, p.q, ext, st, p.Hq / p.Hkv, tokens);
-}
-
-struct PagedLaunch {
-  PagedParams p;
-  CUtensorMap k, v;
-  PagedSplit rows, tiles;
-};
-
-template <int D>
-static int launch_tiles(const PagedLaunch& a) {
-  constexpr int SMEM = 6 * 128 * D * 2 + 1024 + 256;
+template <int D, bool FEW>
+static int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p) {
+  using S = PagedShape<D, FEW>;
   static bool configured[64] = {false};   // per device: kd_shutdown + kd_init may move the library to another GPU
   if (!configured[ctx().device & 63]) {
-    KD_CUDA_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    KD_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_kernel<D, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     configured[ctx().device & 63] = true;
   }
-  const PagedParams& p = a.p;
-  const int per_tile = PA_ROWS / (p.Hq / p.Hkv);
+  // [token][head][D] with a box of the query heads of a tile's tokens on one KV head, 64 channels wide
+  const int group = p.Hq / p.Hkv, blocks = ctx().sm_count;
+  KD_REQUIRE(blocks <= PA_BLOCKS, "%d multiprocessors", blocks);
+  const int64_t ext[4] = {1, p.T, p.Hq, D}, st[3] = {p.T * p.sq_t, p.sq_t, p.sq_h};
   CUtensorMap tq;
-  KD_TRY(make_tmap_heads(&tq, p, per_tile));
-  const int64_t blocks = a.tiles.slots + (int64_t)p.T / (2 * per_tile) + p.B;     // items of all sequences, and one more for every cut
-  KD_CUDA_CHECK(launch_ex(paged_tiles_kernel<D>, dim3((unsigned)blocks, p.Hkv), dim3(PT_THREADS), (size_t)SMEM, tq, a.k, a.v, p, a.tiles));
-  return after_launch("paged_tiles_kernel");
-}
-template <int D, int QROWS>
-static int launch_rows(const PagedLaunch& a) {
-  using S = RowShape<D, QROWS>;
-  static bool configured[64] = {false};
-  if (!configured[ctx().device & 63]) {
-    KD_CUDA_CHECK(cudaFuncSetAttribute(paged_rows_kernel<D, QROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-    configured[ctx().device & 63] = true;
-  }
-  CUtensorMap tq;
-  KD_TRY(make_tmap_heads(&tq, a.p, QROWS / (a.p.Hq / a.p.Hkv)));
-  const dim3 grid(ctx().sm_count), block(PR_THREADS);
-  if (a.p.behind_tiles) KD_CUDA_CHECK(launch_behind(paged_rows_kernel<D, QROWS>, grid, block, (size_t)S::SMEM, tq, a.k, a.v, a.p, a.rows));
-  else KD_CUDA_CHECK(launch_ex(paged_rows_kernel<D, QROWS>, grid, block, (size_t)S::SMEM, tq, a.k, a.v, a.p, a.rows));
-  KD_TRY(after_launch("paged_rows_kernel"));
-  if constexpr (QROWS == PA_ROWS) {
-    KD_CUDA_CHECK(launch_behind(paged_rows_join_kernel<D>, dim3(ctx().sm_count, 4), dim3(256), 0, a.p, a.rows));
-    KD_TRY(after_launch("paged_rows_join_kernel"));
+  KD_TRY(make_tmap_bhsd(&tq, p.q, ext, st, group, S::QROWS / group));
+  const uint64_t places = 2 * (uint64_t)blocks * (FEW ? S::QROWS : 2 * PA_ROWS);
+  void* scratch;
+  KD_TRY(get_workspace(places * (D * 4 + 8) + (uint64_t)blocks * 16, &scratch));
+  PagedSplit out{};
+  out.part_o = static_cast<float*>(scratch);
+  out.part_ml = reinterpret_cast<float2*>(out.part_o + places * D);
+  out.cut = reinterpret_cast<int4*>(out.part_ml + places);
+  KD_CUDA_CHECK(launch_ex(paged_attention_kernel<D, FEW>, dim3(blocks), dim3(PA_THREADS), (size_t)S::SMEM, tq, tk, tv, p, out));
+  KD_TRY(after_launch("paged_attention_kernel"));
+  if constexpr (!FEW) {
+    KD_CUDA_CHECK(launch_behind(paged_join_kernel<D>, dim3(blocks, 2 * PA_ROWS / 32), dim3(256), 0, p, out));
+    KD_TRY(after_launch("paged_join_kernel"));
   }
   return KD_OK;
 }
 
-template <int D>
-static int launch_paged(PagedLaunch& a) {
-  PagedParams& p = a.p;
-  const int64_t rows = (int64_t)p.max_query * (p.Hq / p.Hkv);
-  const bool tiles = rows > PA_ROWS, few = rows <= PA_ROWS || p.q_start;
-  const int sms = ctx().sm_count, part = rows <= 32 ? 32 : PA_ROWS;
-  KD_REQUIRE(sms <= PA_BLOCKS, "%d multiprocessors", sms);
-  a.tiles.slots = sms / p.Hkv > 0 ? sms / p.Hkv : 1;
-  const uint64_t row_places = few ? 2 * (uint64_t)sms * part : 0, tile_places = tiles ? 2 * (uint64_t)a.tiles.slots * p.Hkv * PT_ROWS : 0;
-  void* scratch;
-  KD_TRY(get_workspace((row_places + tile_places) * (D * 4 + 8) + ((uint64_t)sms + a.tiles.slots + 1) * 16, &scratch));
-  a.rows.part_o = static_cast<float*>(scratch);
-  a.tiles.part_o = a.rows.part_o + row_places * D;
-  a.rows.part_ml = reinterpret_cast<float2*>(a.tiles.part_o + tile_places * D);
-  a.tiles.part_ml = a.rows.part_ml + row_places;
-  a.rows.cut = reinterpret_cast<int4*>(a.tiles.part_ml + tile_places);
-  a.tiles.cut = a.rows.cut + sms;
-  a.tiles.cuts = reinterpret_cast<int*>(a.tiles.cut + a.tiles.slots);
-  p.behind_tiles = tiles;
-  if (tiles) KD_TRY(launch_tiles<D>(a));
-  if (few) KD_TRY((rows <= 32 ? launch_rows<D, 32>(a) : launch_rows<D, PA_ROWS>(a)));
-  if (!tiles) return KD_OK;
-  KD_CUDA_CHECK(launch_behind(paged_tiles_join_kernel<D>, dim3(a.tiles.slots, p.Hkv, PT_ROWS / 32), dim3(256), 0, p, a.tiles));
-  return after_launch("paged_tiles_join_kernel");
-}
-
-// After an error a sequence may have been left with some of its parts counted (context.cu, check_device_flag).
+// After an error an item may have been left with some of its parts counted (context.cu, check_device_flag).
 int paged_reset_counters() {
   void* at = nullptr;
   KD_CUDA_CHECK(cudaGetSymbolAddress(&at, g_paged_through));
@@ -1060,8 +852,7 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   }
   KD_REQUIRE(max_query >= 0, "max_query must not be negative");
   if (T == 0 || B == 0) return KD_OK;
-  PagedLaunch a{};
-  PagedParams& p = a.p;
+  PagedParams p{};
   p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.D = D; p.max_pages = max_pages;
   p.pages = (int)k_pool->shape[0];
   p.even = q_start ? 0 : T / B;
@@ -1081,7 +872,10 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   for (int i = 0; i < 3; ++i) { p.sk[i] = k_pool->strides[i]; p.sv[i] = v_pool->strides[i]; }
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = ctx().error_flag;
-  KD_TRY(make_tmap_bhsd(&a.k, p.k, k_pool->shape, k_pool->strides, 128));
-  KD_TRY(make_tmap_bhsd(&a.v, p.v, v_pool->shape, v_pool->strides, 128));
-  return D == 128 ? launch_paged<128>(a) : launch_paged<64>(a);
+  CUtensorMap tk, tv;
+  KD_TRY(make_tmap_bhsd(&tk, p.k, k_pool->shape, k_pool->strides, 128));
+  KD_TRY(make_tmap_bhsd(&tv, p.v, v_pool->shape, v_pool->strides, 128));
+  const bool few = (int64_t)p.max_query * (Hq / Hkv) <= 32;
+  if (D == 128) return few ? launch_paged<128, true>(tk, tv, p) : launch_paged<128, false>(tk, tv, p);
+  return few ? launch_paged<64, true>(tk, tv, p) : launch_paged<64, false>(tk, tv, p);
 }

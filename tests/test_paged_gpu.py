@@ -59,6 +59,21 @@ def test_attention_of_packed_sequences(backend, new, keys, heads, kv_heads, dim)
     assert np.array_equal(run(c, max_query=max(new)), got), "the same call gives the same bits"
 
 
+@pytest.mark.parametrize("most,longest,heads,kv_heads,dim", [(1, 700, 32, 16, 128), (1, 260, 64, 32, 64), (3, 900, 32, 8, 128), (6, 500, 48, 24, 128), (9, 1300, 40, 20, 64), (40, 400, 64, 16, 128),
+                                                             (300, 700, 16, 8, 128), (300, 600, 24, 12, 64), (150, 200, 64, 8, 64)])
+def test_attention_of_many_sequences(backend, most, longest, heads, kv_heads, dim):
+    """Blocks go through many pieces of sequences of all lengths, some without keys or new tokens."""
+    rng = np.random.default_rng(most * longest)
+    count = 60 if most < 100 else 30
+    new = np.minimum(rng.integers(0, most + 1, count) + (rng.random(count) < 0.8), most).tolist()
+    keys = [0 if rng.random() < 0.05 else n + int(k) for n, k in zip(new, rng.integers(0, longest, count) * (rng.random(count) < 0.8))]
+    new[7], keys[7] = most, longest
+    c = attention_case(new, keys, heads, kv_heads, dim, seed=most)
+    got = run(c, max_query=most)
+    check(c, got)
+    assert np.array_equal(run(c, max_query=most), got)
+
+
 @pytest.mark.parametrize("junk", [float("inf"), -3e38])
 def test_attention_ignores_what_stale_rows_hold(backend, junk):
     c = attention_case([1, 40, 150], [70, 300, 1000], 8, 4, 128, junk=junk)
