@@ -271,8 +271,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *q_smem = smem + S::Q_AT, *ring = smem + S::RING_AT;      // (an MMA reads 128 rows: what follows stands in for missing ones)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS_AT);
-  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *o_done = bars + 10, *o_free = bars + 12, *few_done = bars + 13;
-  uint64_t *s_free = bars + 14, *y_bar = bars + 16;     // scores have been loaded [S]; sums of the two chains are there [quarter]
+  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_free = bars + 8;      // scores are there [chain], have been loaded [S]
+  uint64_t *p_ready = bars + 12, *o_done = bars + 14, *o_free = bars + 16, *few_done = bars + 17, *y_bar = bars + 18;      // y_bar: sums of the two chains are there [quarter]
   uint64_t *full = bars + 26, *empty = full + 2 * RING;      // up to 12 each
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);      // and behind it one that stays 0
@@ -287,8 +287,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   const int group = shape.group;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&o_done[i], 1); }
-    for (int i = 0; i < 4; ++i) { mbar_init(&p_ready[i], 4); mbar_init(&y_bar[i], 2); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); }
+    for (int i = 0; i < 4; ++i) mbar_init(&y_bar[i], 2);
     mbar_init(o_free, FEW ? 1 : PA_SOFTMAX);
     mbar_init(few_done, 2);
     for (int i = 0; i < 2 * RING; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -311,13 +311,27 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;      // S of chain t at 128 (t % NS), P at P_COL + 64 t, O at O_COL + D t
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);      // S of chain t at 128 (t % NS), P at P_COL + 64 t, O at O_COL + D t
   pdl_trigger();                              // after the TMEM allocation (see common.cuh)
   Walk walk = *walk_s;
   if (!FEW && threadIdx.x == 0) out.cut[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes what is cut, too)
   Piece w;
   int issued[2] = {0, 0}, q_loaded = 0;       // pages' keys and values and items' queries asked for, by the copying warp
+  auto mbar_test = [](uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+  };
+  // As wait, asking without pause for a while: a step of the chains' loop hangs on it.
+  auto wait_soon = [&](uint64_t* bar, uint32_t parity, int code) {
+    bool ok = false;
+    for (int spins = 0; !ok && spins < 4096; ++spins) ok = __all_sync(0xffffffffu, mbar_test(bar, parity));
+    return ok || (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code));
+  };
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code)); };
+  // Descriptors and addresses pass through a shuffle, which tells the compiler that they are alike in a warp: what was made of numbers read from memory
+  // went through vector registers for every MMA and took 85 cycles each, whatever its size.
+  auto uniform_desc = [](uint32_t addr, uint32_t lbo) { return make_smem_desc_sw128(__shfl_sync(0xffffffffu, addr, 0), lbo, 1024); };
   // where the outputs of a tile's row go
   auto out_row = [&](const SeqWork& s, int hk, int token, int r) { return p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h; };
 
@@ -367,28 +381,26 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // beside the operands that the tensor pipe reads from shared memory, and with ten waits and 32 MMAs for two tiles and a page one
     // warp took 5700 cycles, more than the softmax.  One warp for each chain would not see every phase of the barriers that it waits for.)
     bool ok = true;
-    int page = 0, q_done = 0, uses[2] = {0, 0};      // pages, items with keys, uses of an S
+    int page = 0, q_done = 0, uses[2] = {0, 0};      // pages, items with keys, uses of a chain's S (NS = 1: of both's)
     while (ok && walk.next(p, shape, cache, w)) {
       if (w.nb == 0) continue;
       const int qb = FEW ? q_done & 1 : 0;
       const bool pair = !FEW && w.pair;
       int n[2];
       w.tiles(shape, n);
-      if (!(ok = wait(&q_full[qb], (uint32_t)((FEW ? q_done >> 1 : q_done) & 1), 324))) break;
+      if (!(ok = wait_soon(&q_full[qb], (uint32_t)((FEW ? q_done >> 1 : q_done) & 1), 324))) break;
 #pragma unroll 1
       for (int g = 0; ok && g < w.nb; ++g, ++page) {
         const int slot = page % RING;
-        if (!(ok = wait(&full[slot], (uint32_t)((page / RING) & 1), 325))) break;
+        if (!(ok = wait_soon(&full[slot], (uint32_t)((page / RING) & 1), 325))) break;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (pair ? g >= n[t] : (g & 1) != t) continue;
-          constexpr int last_s = NS - 1;
-          const int sb = t & last_s;
-          if (uses[sb] > 0 && !(ok = wait(&s_free[sb], (uint32_t)((uses[sb] - 1) & 1), 340))) break;      // what was in it has been loaded
-          ++uses[sb];
+          const int sb = NS == 1 ? 0 : t;
+          const uint64_t qdesc = uniform_desc(smem_u32(q_smem + (qb + (pair ? t : 0)) * Q_BYTES), 16), kdesc = uniform_desc(smem_u32(ring + slot * TILE), 16);
+          if (uses[sb] > 0 && !(ok = wait_soon(&s_free[sb], (uint32_t)((uses[sb] - 1) & 1), 340))) break;      // what was in it has been loaded
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t qdesc = make_smem_desc_sw128(smem_u32(q_smem + (qb + (pair ? t : 0)) * Q_BYTES), 16, 1024), kdesc = make_smem_desc_sw128(smem_u32(ring + slot * TILE), 16, 1024);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
               umma_ss(tmem_base + (uint32_t)(sb * 128), qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
@@ -396,6 +408,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             umma_commit(&s_full[t]);
           }
           __syncwarp();
+          if (!ok) break;
+          ++uses[sb];
         }
         if (!ok) break;
         if (elect_one()) {
@@ -416,28 +430,25 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       int n[2];
       w.tiles(shape, n);
       // the sums of the piece before have been read
-      if (q_done > 0 && !(ok = wait(o_free, (uint32_t)((q_done - 1) & 1), 328))) break;
+      if (q_done > 0 && !(ok = wait_soon(o_free, (uint32_t)((q_done - 1) & 1), 328))) break;
 #pragma unroll 1
       for (int g = 0; ok && g < w.nb; ++g, ++page) {
         const int slot = RING + page % RING;
-        if (!(ok = wait(&full[slot], (uint32_t)((page / RING) & 1), 326))) break;
+        if (!(ok = wait_soon(&full[slot], (uint32_t)((page / RING) & 1), 326))) break;
 #pragma unroll
         for (int t = 0; ok && t < 2; ++t) {
           if (pair ? g >= n[t] : (g & 1) != t) continue;
+          const uint64_t vdesc = uniform_desc(smem_u32(ring + slot * TILE), SLAB);
+          const uint32_t more = __shfl_sync(0xffffffffu, (pair ? g : g >> 1) != 0 ? 1u : 0u, 0);
+          if (!(ok = wait_soon(&p_ready[t], (uint32_t)(turn[t] & 1), 327))) break;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (!(ok = wait(&p_ready[2 * t + half], (uint32_t)(turn[t] & 1), 327))) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t vdesc = make_smem_desc_sw128(smem_u32(ring + slot * TILE), SLAB, 1024);
-#pragma unroll
-              for (int k = 4 * half; k < 4 * half + 4; ++k)
-                umma_ts(tmem_base + O_COL + (uint32_t)(t * D), tmem_base + P_COL + (uint32_t)(t * 64 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV,
-                        ((pair ? g : g >> 1) | k) != 0 ? 1u : 0u);
-              if (half == 1) umma_commit(&o_done[t]);
-            }
-            __syncwarp();
+            for (int k = 0; k < 8; ++k)
+              umma_ts(tmem_base + O_COL + (uint32_t)(t * D), tmem_base + P_COL + (uint32_t)(t * 64 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV, k != 0 ? 1u : more);
+            umma_commit(&o_done[t]);
           }
+          __syncwarp();
           ++turn[t];
         }
         if (!ok) break;
@@ -539,30 +550,45 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       const int mine = t ? n[1] : n[0];
       int my_turn = t ? turns[1] : turns[0];
       float m = -1e30f, l = 0.f;
+      // P, and values that were cleared, are there for the product
+      auto hand_over = [&] {
+        if (active) tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[t]);
+      };
       for (int i = 0; i < mine; ++i, ++my_turn) {
         const int g = pair ? i : 2 * i + t, kv0 = (w.j0 + g) * 128;
+        uint32_t r[128];
+        float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f;
+        const bool masked = kv0 + 127 > hidden;                     // some row does not see all of these keys
+        const int lim = last - kv0;
+        // P of the tile before is handed over when its store is done: while the scores are waited for, or else behind their load
+        bool handed = i == 0;
+        if (!handed && !__all_sync(0xffffffffu, mbar_test(&s_full[t], (uint32_t)(my_turn & 1)))) {
+          hand_over();
+          handed = true;
+        }
         if (!(ok = wait(&s_full[t], (uint32_t)(my_turn & 1), 329))) break;
         tc_fence_after();
-        uint32_t r[128];
         if (active) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r + c * 32);
-          tmem_wait_ld();
         }
+        if (!handed) hand_over();
+        if (active) tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t % NS]);
+        if (lane == 0) mbar_arrive(&s_free[NS == 1 ? 0 : t]);
         float alpha = 1.f;
         bool rescale = false;
         float neg_m = 0.f;
         if (active) {
-          if (kv0 + 127 > hidden) {                                 // some row does not see all of these keys
-            const int lim = last - kv0;
+          if (masked) {
 #pragma unroll
             for (int e = 0; e < 128; ++e)
               if (e > lim) r[e] = __float_as_uint(-1e30f);
           }
-          float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f;
 #pragma unroll
           for (int e = 0; e < 128; e += 8) {
             mx0 = pa_max3(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
@@ -581,62 +607,55 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           neg_m = -m;
         }
-        // P = 2^(s c - m) as packed bf16, handed over in two halves of 64 keys.  (Probabilities meet the values as bf16, the type of the
-        // tensor cores' other operand; their sum stays in fp32.)
+        // P = 2^(s c - m) as packed bf16.  (Probabilities meet the values as bf16, the type of the tensor cores' other operand; their sum stays in
+        // fp32.)
         float sum0 = 0.f, sum1 = 0.f;
+        if (active) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (active) {
-#pragma unroll
-            for (int e = 32 * half; e < 32 * half + 32; ++e) {
-              float x0, x1;
-              pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), p.scale_log2, neg_m);
-              const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
-              pa_add2(sum0, sum1, e0, e1);
-              r[e] = pack_bf16(e0, e1);
-            }
+          for (int e = 0; e < 64; ++e) {
+            float x0, x1;
+            pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), p.scale_log2, neg_m);
+            const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
+            pa_add2(sum0, sum1, e0, e1);
+            r[e] = pack_bf16(e0, e1);
           }
-          if (half == 0) {
-            // the product before has read P, and O is complete
-            if (my_turn > 0 && !(ok = wait(&o_done[t], (uint32_t)((my_turn - 1) & 1), 332))) break;
-            if (active && __any_sync(0xffffffffu, rescale)) {
-              tc_fence_after();
+        }
+        // the product before has read P, and O is complete
+        if (my_turn > 0 && !(ok = wait(&o_done[t], (uint32_t)((my_turn - 1) & 1), 332))) break;
+        if (active && __any_sync(0xffffffffu, rescale)) {
+          tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D; c += 16) {                     // narrow pieces: the scores stay in registers meanwhile
-                uint32_t o[16];
-                tmem_ld_32x16(o_addr + c, o);
-                tmem_wait_ld();
+          for (int c = 0; c < D; c += 16) {                     // narrow pieces: the scores stay in registers meanwhile
+            uint32_t o[16];
+            tmem_ld_32x16(o_addr + c, o);
+            tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                tmem_st_32x16(o_addr + c, o);
-              }
-              l *= alpha;
-            }
-            if (kv0 + 128 > w.s.ctx && (!pair || t == 0 || i >= n[0])) {
-              // Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them (by
-              // the chain whose product comes first).
-              // (what stood in the slot before has been used, so that the parity is that of this page)
-              if (i == 0 && pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
-              const int slot = RING + (done + g) % RING;
-              if (!(ok = wait(&full[slot], (uint32_t)(((done + g) / RING) & 1), 330))) break;
-              if (kv0 + row >= w.s.ctx) {
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st_32x16(o_addr + c, o);
+          }
+          l *= alpha;
+        }
+        if (kv0 + 128 > w.s.ctx && (!pair || t == 0 || i >= n[0])) {
+          // Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them (by
+          // the chain whose product comes first).
+          // (what stood in the slot before has been used, so that the parity is that of this page)
+          if (i == 0 && pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
+          const int slot = RING + (done + g) % RING;
+          if (!(ok = wait(&full[slot], (uint32_t)(((done + g) / RING) & 1), 330))) break;
+          if (kv0 + row >= w.s.ctx) {
 #pragma unroll
-                for (int d = 0; d < D / 8; ++d) *reinterpret_cast<uint4*>(ring + slot * TILE + (d / 8) * SLAB + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
-              }
-              fence_async_proxy();
-            }
+            for (int d = 0; d < D / 8; ++d) *reinterpret_cast<uint4*>(ring + slot * TILE + (d / 8) * SLAB + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
-          if (active) {
-            tmem_st_32x32(p_addr + half * 32, r + half * 32);
-            tmem_wait_st();
-            tc_fence_before();
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_ready[2 * t + half]);
+          fence_async_proxy();
+        }
+        if (active) {
+          tmem_st_32x32(p_addr, r);
+          tmem_st_32x32(p_addr + 32, r + 32);
         }
         if (!ok) break;
         l += sum0 + sum1;
       }
+      if (ok && mine > 0) hand_over();
       if (!ok) break;
       done += w.nb;
       turns[0] += n[0];
