@@ -61,6 +61,7 @@ constexpr int PA_ROWS = 128;            // rows of a tile
 constexpr int PA_SOFTMAX = 8;           // warps 0-7: chain warp / 4, rows 32 (warp % 4) and on
 constexpr int PA_THREADS = 384;
 constexpr int PA_CACHE = 64;            // sequences whose lengths are kept in shared memory
+constexpr int PA_PIECES = 4;            // pieces of work that the warps of a block may be apart
 
 __device__ __forceinline__ float pa_exp2(float x) {
   float y;
@@ -130,10 +131,11 @@ struct Piece {
     }
   }
 };
-// Goes through the pieces of a block; the same in every warp.
+// Goes through the pieces of a block.
 struct Walk {
   int64_t u, end, per;
-  int b, hk, item, off;
+  int b, hk, item, off, block;
+  __device__ __forceinline__ int quotient(int64_t x) const { return (x | per) >> 32 ? (int)(x / per) : (int)((uint32_t)x / (uint32_t)per); }
   __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape& shape, const int4* cache, Piece& w) {
     if (u >= end) return false;
     for (;;) {
@@ -152,9 +154,9 @@ struct Walk {
     w.b = b; w.hk = hk; w.item = item;
     w.j0 = min(off / weight, pages);
     w.nb = min((off + take) / weight, pages) - w.j0;
-    w.first = (int)(start / per);
-    w.parts = (int)((start + all - 1) / per) - w.first + 1;
-    w.part = (int)(u / per) - w.first;
+    w.first = off ? quotient(start) : block;
+    w.parts = (start + all <= end ? block : quotient(start + all - 1)) - w.first + 1;
+    w.part = block - w.first;
     u += take;
     off = 0;
     ++item;
@@ -178,6 +180,7 @@ __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape
   w.u = min(all, x * w.per);
   w.end = min(all, w.u + w.per);
   w.hk = w.b = w.item = w.off = 0;
+  w.block = x;
   if (w.u >= w.end) return w;
   w.hk = (int)(w.u / sum);
   int64_t left = w.u - w.hk * sum;
@@ -249,11 +252,14 @@ struct PagedShape {
   static constexpr int TILE = 128 * D * 2, RING = (FEW ? 3 : 2) * 32768 / TILE;      // slots for keys, and as many for values
   static constexpr int QROWS = FEW ? 32 : PA_ROWS, Q_BYTES = QROWS * D * 2;
   static constexpr int Q_AT = 0, RING_AT = 2 * Q_BYTES, BARS_AT = RING_AT + 2 * RING * TILE;
-  static constexpr int CACHE_AT = BARS_AT + 640, ML_AT = CACHE_AT + PA_CACHE * 16, BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
+  static constexpr int CACHE_AT = BARS_AT + 1024, ML_AT = CACHE_AT + PA_CACHE * 16, BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
   // tensor memory: scores, probabilities, sums
   static constexpr int NS = D == 128 ? 1 : 2;
   static constexpr uint32_t P_COL = 128 * NS, O_COL = P_COL + 128;
   static_assert(O_COL + 2 * D == 512, "tensor memory has 512 columns");
+  // registers of a thread of warps 8-11 and of the others: the outputs' warp needs its own, else the scores do
+  static constexpr int OTHER_REGS = FEW ? 120 : 72, SOFTMAX_REGS = FEW ? 192 : 216;
+  static_assert((PA_THREADS - PA_SOFTMAX * 32) * OTHER_REGS + PA_SOFTMAX * 32 * SOFTMAX_REGS <= PA_THREADS * 168, "registers of the launch");
   static constexpr int SMEM = BYTES + 1024;
   static_assert(SMEM <= 227 * 1024, "tiles exceed shared memory");
 };
@@ -277,45 +283,47 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);      // and behind it one that stays 0
   int* joins = const_cast<int*>(abort_flag) + 2;                                  // items that this block joins at the end
-  Walk* walk_s = reinterpret_cast<Walk*>(bars + 52);
-  Piece* join_s = reinterpret_cast<Piece*>(walk_s + 1);                           // [2]
-  static_assert(52 * 8 + sizeof(Walk) + 2 * sizeof(Piece) <= 640, "barriers and what stands behind them");
+  uint64_t *piece_full = bars + 52, *piece_empty = piece_full + PA_PIECES;
+  Piece* piece_s = reinterpret_cast<Piece*>(piece_empty + PA_PIECES);             // what the warps work on; no parts: behind the last one
+  Piece* join_s = piece_s + PA_PIECES;                                            // [2]
+  static_assert((52 + 2 * PA_PIECES) * 8 + (PA_PIECES + 2) * sizeof(Piece) <= 1024, "barriers and what stands behind them");
   int4* cache = reinterpret_cast<int4*>(smem + S::CACHE_AT);
   float2* ml = reinterpret_cast<float2*>(smem + S::ML_AT);     // [piece & 1][chain][row] (maximum, sum)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const ItemShape shape{p.Hq / p.Hkv, QROWS / (p.Hq / p.Hkv)};
   const int group = shape.group;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); }
-    for (int i = 0; i < 4; ++i) mbar_init(&y_bar[i], 2);
-    mbar_init(o_free, FEW ? 1 : PA_SOFTMAX);
-    mbar_init(few_done, 2);
-    for (int i = 0; i < 2 * RING; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    abort_flag[0] = abort_flag[1] = 0;
-    *joins = 0;
-    fence_mbar_init();
-    prefetch_tmap(&tmap_q);
-    prefetch_tmap(&tmap_k);
-    prefetch_tmap(&tmap_v);
-  }
-  if (warp == 10) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  pdl_wait();
+  // The copying warp sets up the barriers and goes on; the others meet it at a barrier that it only arrives at.
   if (warp == 9) {
-    const Walk w = paged_walk(p, shape, blockIdx.x, gridDim.x, cache);
-    if (lane == 0) *walk_s = w;
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); }
+      for (int i = 0; i < 4; ++i) mbar_init(&y_bar[i], 2);
+      mbar_init(o_free, FEW ? 1 : PA_SOFTMAX);
+      mbar_init(few_done, 2);
+      for (int i = 0; i < 2 * RING; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+      for (int i = 0; i < PA_PIECES; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], PA_SOFTMAX + 2 + (FEW ? 1 : 0)); }
+      abort_flag[0] = abort_flag[1] = 0;
+      *joins = 0;
+      fence_mbar_init();
+      prefetch_tmap(&tmap_q);
+      prefetch_tmap(&tmap_k);
+      prefetch_tmap(&tmap_v);
+    }
+    __syncwarp();
+    asm volatile("bar.arrive 3, %0;" ::"n"(PA_THREADS) : "memory");
+  } else {
+    if (warp == 10) {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+      tc_fence_before();
+    }
+    asm volatile("bar.sync 3, %0;" ::"n"(PA_THREADS) : "memory");
   }
-  tc_fence_before();
-  __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);      // S of chain t at 128 (t % NS), P at P_COL + 64 t, O at O_COL + D t
-  pdl_trigger();                              // after the TMEM allocation (see common.cuh)
-  Walk walk = *walk_s;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, warp == 9 ? 0u : *tmem_slot, 0);      // (warp 9 may be ahead of it)  S of chain t at 128 (t % NS), P at P_COL + 64 t, O at O_COL + D t
+  pdl_wait();
+  if (warp == 10) pdl_trigger();              // after the TMEM allocation (see common.cuh): one thread's is the block's
   if (!FEW && threadIdx.x == 0) out.cut[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes what is cut, too)
-  Piece w;
   int issued[2] = {0, 0}, q_loaded = 0;       // pages' keys and values and items' queries asked for, by the copying warp
   auto mbar_test = [](uint64_t* bar, uint32_t parity) {
     uint32_t done;
@@ -329,6 +337,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     return ok || (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code));
   };
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code)); };
+  // The k-th piece of the block's share, and that the warp is done with it.  nullptr: there are no more, or a wait ran out.
+  auto piece_at = [&](int k) -> const Piece* {
+    if (!wait(&piece_full[k % PA_PIECES], (uint32_t)((k / PA_PIECES) & 1), 341)) return nullptr;
+    return piece_s[k % PA_PIECES].parts ? piece_s + k % PA_PIECES : nullptr;
+  };
+  auto piece_done = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&piece_empty[k % PA_PIECES]);
+  };
   // Descriptors and addresses pass through a shuffle, which tells the compiler that they are alike in a warp: what was made of numbers read from memory
   // went through vector registers for every MMA and took 85 cycles each, whatever its size.
   auto uniform_desc = [](uint32_t addr, uint32_t lbo) { return make_smem_desc_sw128(__shfl_sync(0xffffffffu, addr, 0), lbo, 1024); };
@@ -336,10 +353,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   auto out_row = [&](const SeqWork& s, int hk, int token, int r) { return p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h; };
 
   if (warp >= PA_SOFTMAX) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER_REGS));
   if (warp == 9) {
+    // This warp alone goes through the division: its state does not fit beside the others' registers, and each began a piece some 4000 cycles late.
+    Walk walk = paged_walk(p, shape, blockIdx.x, gridDim.x, cache);
     bool ok = true;
-    while (ok && walk.next(p, shape, cache, w)) {
+    for (int k = 0; ok; ++k) {
+      Piece w;
+      const bool more = walk.next(p, shape, cache, w);
+      if (!more) w.parts = 0;
+      if (!wait(&piece_empty[k % PA_PIECES], (uint32_t)(((k / PA_PIECES) & 1) ^ 1), 342)) break;
+      if (lane == 0) {
+        piece_s[k % PA_PIECES] = w;
+        mbar_arrive(&piece_full[k % PA_PIECES]);
+      }
+      __syncwarp();
+      if (!more) break;
       if (w.nb == 0) continue;
       int page = lane < w.nb ? p.table[w.b * p.table_row + w.j0 + lane] : 0;      // 32 entries of the table at a time
       // queries: one item's two tiles, or FEW: two items' one tile
@@ -382,7 +411,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // warp took 5700 cycles, more than the softmax.  One warp for each chain would not see every phase of the barriers that it waits for.)
     bool ok = true;
     int page = 0, q_done = 0, uses[2] = {0, 0};      // pages, items with keys, uses of a chain's S (NS = 1: of both's)
-    while (ok && walk.next(p, shape, cache, w)) {
+    for (int k = 0; ok; ++k) {
+      const Piece* at = piece_at(k);
+      if (!at) break;
+      const Piece w = *at;
+      piece_done(k);
       if (w.nb == 0) continue;
       const int qb = FEW ? q_done & 1 : 0;
       const bool pair = !FEW && w.pair;
@@ -424,7 +457,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // Products: O_t += P_t V(g), in the same order.
     bool ok = true;
     int page = 0, q_done = 0, turn[2] = {0, 0};      // pages, items with keys, tiles of a chain
-    while (ok && walk.next(p, shape, cache, w)) {
+    for (int k = 0; ok; ++k) {
+      const Piece* at = piece_at(k);
+      if (!at) break;
+      const Piece w = *at;
+      piece_done(k);
       if (w.nb == 0) continue;
       const bool pair = !FEW && w.pair;
       int n[2];
@@ -461,7 +498,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // Outputs of pieces with up to 32 rows, while the chains go on.
     int pieces = 0, turns[2] = {0, 0};
     bool ok = true;
-    while (ok && walk.next(p, shape, cache, w)) {
+    for (int k = 0; ok; ++k) {
+      const Piece* piece = piece_at(k);
+      if (!piece) break;
+      const Piece w = *piece;
+      piece_done(k);
       const int rows = w.s.n * group;
       const bool real = lane < rows, direct = w.parts == 1;
       float f[2] = {0.f, 0.f}, M = -1e30f, L = 0.f;
@@ -488,36 +529,38 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       __nv_bfloat16* to = real ? out_row(w.s, w.hk, lane / group, lane) : nullptr;
       const int64_t at = (int64_t)(2 * blockIdx.x + (w.part == 0 ? 1 : 0)) * QROWS + lane;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        float o[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (!use[k]) continue;
-          uint32_t x[16];
+      for (int c = 0; c < D; c += 32) {
+        uint32_t x[64];
+        __syncwarp();
+        if (use[0]) tmem_ld_32x32(tmem_base + O_COL + c, x);
+        if (use[1]) tmem_ld_32x32(tmem_base + O_COL + D + c, x + 32);
+        tmem_wait_ld();
+        if (c + 32 == D && w.nb > 0) {
+          tc_fence_before();
           __syncwarp();
-          tmem_ld_32x16(tmem_base + O_COL + k * D + c, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = f[k] == 0.f ? o[e] : fmaf(f[k], __uint_as_float(x[e]), o[e]);
+          if (lane == 0) mbar_arrive(o_free);
         }
-        if (real && direct) {
+        if (!real) continue;
 #pragma unroll
-          for (int e = 0; e < 16; e += 8)
-            *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]), pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
-        } else if (real) {
+        for (int e = 0; e < 32; e += 8) {
+          float o[8];
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(out.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int k = 0; k < 8; ++k) {
+            o[k] = f[0] == 0.f ? 0.f : f[0] * __uint_as_float(x[e + k]);
+            if (f[1] != 0.f) o[k] = fmaf(f[1], __uint_as_float(x[32 + e + k]), o[k]);
+          }
+          if (direct) {
+            *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+          } else {
+            float4* part = reinterpret_cast<float4*>(out.part_o + at * D + c + e);
+            part[0] = make_float4(o[0], o[1], o[2], o[3]);
+            part[1] = make_float4(o[4], o[5], o[6], o[7]);
+          }
         }
       }
       if (real && !direct) out.part_ml[at] = make_float2(M, L);
-      tc_fence_before();
       __syncwarp();
-      if (w.nb > 0) {
-        ++pieces;
-        if (lane == 0) mbar_arrive(o_free);
-      }
+      if (w.nb > 0) ++pieces;
       if (!direct && lane == 0) {
         // the part that is through last joins them all, at the end of its block (in the parts' order, whoever is last)
         unsigned before;
@@ -532,13 +575,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFTMAX_REGS));
     const int t = warp >> 2, q = warp & 3, row = q * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)(t % NS * 128), p_addr = lane_addr + P_COL + (uint32_t)(t * 64), o_addr = lane_addr + O_COL + (uint32_t)(t * D);
     const int row_token = row / group;
     int done = 0, pieces = 0, turns[2] = {0, 0}, y_turn = 0;
     bool ok = true;
-    while (ok && walk.next(p, shape, cache, w)) {
+    for (int k = 0; ok; ++k) {
+      const Piece* piece = piece_at(k);
+      if (!piece) break;
+      const Piece& w = *piece;                                      // (not copied: the registers are for scores)
       const bool pair = !FEW && w.pair;
       // this chain's tile
       const int token0 = pair ? (2 * w.item + t) * shape.tokens : 0, tokens = min(shape.tokens, w.s.n - token0), rows = tokens * group;
@@ -665,7 +711,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (mine == 0 || last < first_key) { m = -1e30f; l = 0.f; }
       float2* now = ml + (pieces & 1) * 2 * PA_ROWS;
       if constexpr (FEW) {
-        if (w.nb == 0) continue;
+        const bool some = w.nb > 0;
+        piece_done(k);
+        if (!some) continue;
         if (q == 0) {
           // (the outputs of the piece before have been read: nobody is two pieces ahead)
           if (pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
@@ -705,39 +753,42 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (n[1] > 0 && !(pair && t == 0) && !(ok = wait(&o_done[1], (uint32_t)((turns[1] - 1) & 1), 336))) break;
         tc_fence_after();
       }
+      // this warp's channels: its own chain's, or half of both chains'
+      const bool some = w.nb > 0;
       if (active) {
-        // this warp's channels: its own chain's, or half of both chains'
         const int width = pair ? D : D / 2, c0 = pair ? 0 : t * width;
-        const bool use[2] = {w.nb > 0 && n[0] > 0 && !(pair && t == 1), w.nb > 0 && n[1] > 0 && !(pair && t == 0)};
-        __nv_bfloat16* to = real ? out_row(w.s, w.hk, token0 + row_token, row) : nullptr;
+        const bool use[2] = {some && n[0] > 0 && !(pair && t == 1), some && n[1] > 0 && !(pair && t == 0)};
+        __nv_bfloat16* to = out_row(w.s, w.hk, token0 + row_token, row);
         const int64_t at = (int64_t)place * (2 * PA_ROWS) + (pair ? t * PA_ROWS : 0) + row;
 #pragma unroll 1
         for (int c = c0; c < c0 + width; c += 16) {
-          float o[16];
+          uint32_t x[32];
+          __syncwarp();
+          if (use[0]) tmem_ld_32x16(lane_addr + O_COL + c, x);
+          if (use[1]) tmem_ld_32x16(lane_addr + O_COL + D + c, x + 16);
+          tmem_wait_ld();
+          if (!real) continue;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+          for (int e = 0; e < 16; e += 8) {
+            float o[8];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (!use[k]) continue;                                  // (alike in a whole warp)
-            uint32_t x[16];
-            __syncwarp();
-            tmem_ld_32x16(lane_addr + O_COL + k * D + c, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = f[k] == 0.f ? o[e] : fmaf(f[k], __uint_as_float(x[e]), o[e]);
-          }
-          if (real && direct) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 8)
-              *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]), pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
-          } else if (real) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(out.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int i = 0; i < 8; ++i) {
+              o[i] = f[0] == 0.f ? 0.f : f[0] * __uint_as_float(x[e + i]);      // (a share of 0: nothing was written there)
+              if (f[1] != 0.f) o[i] = fmaf(f[1], __uint_as_float(x[16 + e + i]), o[i]);
+            }
+            if (direct) {
+              *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+            } else if (some) {
+              float4* part = reinterpret_cast<float4*>(out.part_o + at * D + c + e);
+              part[0] = make_float4(o[0], o[1], o[2], o[3]);
+              part[1] = make_float4(o[4], o[5], o[6], o[7]);
+            }
           }
         }
         if (real && !direct && (pair || t == 0)) out.part_ml[at] = make_float2(M, L);
       }
-      if (w.nb == 0) continue;
+      piece_done(k);
+      if (!some) continue;
       // (nobody counts twice in a phase: the piece before is over)
       if (pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
       ++pieces;
