@@ -357,20 +357,29 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   if (warp == 9) {
     // This warp alone goes through the division: its state does not fit beside the others' registers, and each began a piece some 4000 cycles late.
     Walk walk = paged_walk(p, shape, blockIdx.x, gridDim.x, cache);
-    bool ok = true;
-    for (int k = 0; ok; ++k) {
+    int page_first = 0;                                             // the next piece's first 32 entries of the table
+    auto publish = [&](int k) {
       Piece w;
       const bool more = walk.next(p, shape, cache, w);
-      if (!more) w.parts = 0;
-      if (!wait(&piece_empty[k % PA_PIECES], (uint32_t)(((k / PA_PIECES) & 1) ^ 1), 342)) break;
+      if (!more) w.parts = w.nb = 0;
+      if (!wait(&piece_empty[k % PA_PIECES], (uint32_t)(((k / PA_PIECES) & 1) ^ 1), 342)) return false;
       if (lane == 0) {
         piece_s[k % PA_PIECES] = w;
         mbar_arrive(&piece_full[k % PA_PIECES]);
       }
       __syncwarp();
-      if (!more) break;
-      if (w.nb == 0) continue;
-      int page = lane < w.nb ? p.table[w.b * p.table_row + w.j0 + lane] : 0;      // 32 entries of the table at a time
+      if (lane < w.nb) page_first = p.table[w.b * p.table_row + w.j0 + lane];
+      return true;
+    };
+    bool ok = publish(0);
+    for (int k = 0; ok; ++k) {
+      const Piece w = piece_s[k % PA_PIECES];
+      if (!w.parts) break;
+      if (w.nb == 0) {
+        ok = publish(k + 1);
+        continue;
+      }
+      int page = 0, page_next = page_first;                         // entries of the table, 32 at a time
       // queries: one item's two tiles, or FEW: two items' one tile
       const int qb = FEW ? q_loaded & 1 : 0;
       if (!wait(&q_empty[qb], (uint32_t)(((FEW ? q_loaded >> 1 : q_loaded) & 1) ^ 1), 321)) break;
@@ -384,9 +393,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       __syncwarp();
       ++q_loaded;
+      // What is read behind the copies waits for them (three pages of them take some 8000 cycles): the next piece's entries come before them.
+      if (!(ok = publish(k + 1))) break;
       for (int j = 0; j < w.nb; ++j) {
         if (j % 32 == 0) {
-          if (j) page = j + lane < w.nb ? p.table[w.b * p.table_row + w.j0 + j + lane] : 0;
+          page = j + lane < w.nb ? page_next : 0;
+          if (j + 32 + lane < w.nb) page_next = p.table[w.b * p.table_row + w.j0 + j + 32 + lane];
           if ((unsigned)page >= (unsigned)p.pages && atomicCAS(p.err, 0, 103) == 0) { p.err[1] = w.b; p.err[2] = page; }
         }
         const int where = __shfl_sync(0xffffffffu, page, j % 32);
