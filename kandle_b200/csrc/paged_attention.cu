@@ -212,7 +212,7 @@ __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape
 // ----------------------------------------------------------------------------- sums of items that are cut
 // Block x leaves the end of an item that began before it at place 2 x, and the beginning of one that goes on behind it at 2 x + 1.
 struct PagedSplit {
-  float* part_o;      // [place][rows][D] unnormalised sums
+  float* part_o;      // [place][rows][D] unnormalised sums, or [place][D / 4][rows][4] of items with two tiles
   float2* part_ml;    // [place][rows] (running maximum in the log2 domain, sum)
   int4* cut;          // what began in block x and went on: (sequence, KV head, item, parts)
 };
@@ -220,16 +220,27 @@ struct PagedSplit {
 constexpr int PA_BLOCKS = 1024;
 static __device__ unsigned g_paged_through[PA_BLOCKS];
 
+// Where the four channels from c on of a row stand in a place, in float4s.  A thread has a row: with two tiles' 256 rows whole warps store, in one
+// piece if rows stand side by side (1 x 512 tokens on 16384: 96.3 -> 93.1 us); of few rows, the channels are read side by side (8 x 9 tokens:
+// 57.5 us with rows side by side, 53.5 so).
+template <int D>
+__device__ __forceinline__ int part_at(bool pair, int r, int c) { return pair ? c / 4 * (2 * PA_ROWS) + r : r * (D / 4) + c / 4; }
+// The n-th row and four channels of an item to join, in the same order.
+template <int D>
+__device__ __forceinline__ void part_nth(bool pair, int n, int& r, int& c) {
+  r = pair ? n / (2 * D) * 8 + n % 8 : n / (D / 4);
+  c = pair ? n % (2 * D) / 8 * 4 : n % (D / 4) * 4;
+}
 // Four channels of a row from all parts of an item: sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
 template <int D>
-__device__ __forceinline__ void join_parts(const PagedSplit& in, int part_rows, int r, int c, int first, int parts, __nv_bfloat16* to) {
+__device__ __forceinline__ void join_parts(const PagedSplit& in, int part_rows, bool pair, int r, int c, int first, int parts, __nv_bfloat16* to) {
   float m = -1e30f, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int k = 0; k < parts; ++k) {
     const int64_t at = (int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * part_rows + r;
     const float2 x = __ldcg(in.part_ml + at);
-    const float4 o = __ldcg(reinterpret_cast<const float4*>(in.part_o + at * D + c));
+    const float4 o = __ldcg(reinterpret_cast<const float4*>(in.part_o) + (at - r) * (D / 4) + part_at<D>(pair, r, c));
     const float now = fmaxf(m, x.x), f0 = pa_exp2(m - now), f1 = pa_exp2(x.x - now);
     const bool some = x.y != 0.f;        // (else nothing was seen there, and nothing written)
     m = now;
@@ -771,7 +782,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         const int width = pair ? D : D / 2, c0 = pair ? 0 : t * width;
         const bool use[2] = {some && n[0] > 0 && !(pair && t == 1), some && n[1] > 0 && !(pair && t == 0)};
         __nv_bfloat16* to = out_row(w.s, w.hk, token0 + row_token, row);
-        const int64_t at = (int64_t)place * (2 * PA_ROWS) + (pair ? t * PA_ROWS : 0) + row;
+        const int part_row = (pair ? t * PA_ROWS : 0) + row;
+        float4* parts = reinterpret_cast<float4*>(out.part_o) + (int64_t)place * (2 * PA_ROWS * D / 4);
 #pragma unroll 1
         for (int c = c0; c < c0 + width; c += 16) {
           uint32_t x[32];
@@ -791,13 +803,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (direct) {
               *reinterpret_cast<uint4*>(to + c + e) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
             } else if (some) {
-              float4* part = reinterpret_cast<float4*>(out.part_o + at * D + c + e);
+              float4* part = parts + part_at<D>(pair, part_row, c + e);
               part[0] = make_float4(o[0], o[1], o[2], o[3]);
-              part[1] = make_float4(o[4], o[5], o[6], o[7]);
+              part[pair ? 2 * PA_ROWS : 1] = make_float4(o[4], o[5], o[6], o[7]);
             }
           }
         }
-        if (real && !direct && (pair || t == 0)) out.part_ml[at] = make_float2(M, L);
+        if (real && !direct && (pair || t == 0)) out.part_ml[(int64_t)place * (2 * PA_ROWS) + part_row] = make_float2(M, L);
       }
       piece_done(k);
       if (!some) continue;
@@ -822,8 +834,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     for (int i = 0; i < *joins; ++i) {
       const Piece& j = join_s[i];
       for (int n = threadIdx.x; n < j.s.n * group * (D / 4); n += PA_THREADS) {
-        const int r = n / (D / 4);
-        join_parts<D>(out, QROWS, r, n % (D / 4) * 4, j.first, j.parts, out_row(j.s, j.hk, r / group, r));
+        int r, c;
+        part_nth<D>(false, n, r, c);
+        join_parts<D>(out, QROWS, false, r, c, j.first, j.parts, out_row(j.s, j.hk, r / group, r));
       }
     }
   }
@@ -846,9 +859,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   const PagedSeq s = paged_seq(p, c.x);
   const bool pair = shape.pair(s.n);
   for (int n = threadIdx.x; n < 32 * (D / 4); n += 256) {
-    const int r = blockIdx.y * 32 + n / (D / 4), i = (pair ? (2 * c.z + r / PA_ROWS) * shape.tokens : 0) + r % PA_ROWS / shape.group;
+    int r, ch;
+    part_nth<D>(pair, n, r, ch);
+    r += blockIdx.y * 32;
+    const int i = (pair ? (2 * c.z + r / PA_ROWS) * shape.tokens : 0) + r % PA_ROWS / shape.group;
     if (r % PA_ROWS >= shape.tokens * shape.group || i >= s.n || (!pair && r >= PA_ROWS)) continue;
-    join_parts<D>(in, 2 * PA_ROWS, r, n % (D / 4) * 4, blockIdx.x, c.w, p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)(c.y * shape.group + r % PA_ROWS % shape.group) * p.so_h);
+    join_parts<D>(in, 2 * PA_ROWS, pair, r, ch, blockIdx.x, c.w, p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)(c.y * shape.group + r % PA_ROWS % shape.group) * p.so_h);
   }
 }
 
