@@ -16,8 +16,12 @@
 //
 // Softmax.  A thread owns a row and loads its 128 scores at once; S is free from then on, so that the next Q K^T runs beside the exponentials
 // (with P over S it waited for P V, and a chain's step was the sum of both: 4331 cycles for two tiles and a page, of which the exponential unit
-// needs 2048 and the tensor pipe 2048).  With heads of 128 tensor memory holds one S for both chains, which they use in turn, two P and two O; with heads of 64
-// two of each.  Two threads a row (and 16 warps) were slower: they have to exchange the maximum.
+// needs 2048 and the tensor pipe 2048).  Tensor memory holds one S for both chains, which they use in turn, two P and two O.  Two threads a
+// row (and 16 warps) were slower: they have to exchange the maximum.
+//
+// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 85 us, 4.45 TB/s, of which some 25 are the launch, the division,
+// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8) 54 us; 4 x 2048 tokens on 6144 (32 on 8) 1007 us, 955
+// TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
 #include "common.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
@@ -265,9 +269,10 @@ struct PagedShape {
   static constexpr int Q_AT = 0, RING_AT = 2 * Q_BYTES, BARS_AT = RING_AT + 2 * RING * TILE;
   static constexpr int CACHE_AT = BARS_AT + 1024, ML_AT = CACHE_AT + PA_CACHE * 16, BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
   // tensor memory: scores, probabilities, sums
-  static constexpr int NS = D == 128 ? 1 : 2;
-  static constexpr uint32_t P_COL = 128 * NS, O_COL = P_COL + 128;
-  static_assert(O_COL + 2 * D == 512, "tensor memory has 512 columns");
+  // (One buffer for the scores of both chains.  With heads of 64 there is room for two; the chains' softmaxes then run side by side, both at their
+  // exponentials and both not, and a step takes 4400 cycles in place of 4000: 73.8 us against 71.2 in a batch of 12 x 700 tokens.)
+  static constexpr uint32_t P_COL = 128, O_COL = P_COL + 128;
+  static_assert(O_COL + 2 * D <= 512, "tensor memory has 512 columns");
   // registers of a thread of warps 8-11 and of the others: the outputs' warp needs its own, else the scores do
   static constexpr int OTHER_REGS = FEW ? 120 : 72, SOFTMAX_REGS = FEW ? 192 : 216;
   static_assert((PA_THREADS - PA_SOFTMAX * 32) * OTHER_REGS + PA_SOFTMAX * 32 * SOFTMAX_REGS <= PA_THREADS * 168, "registers of the launch");
@@ -281,14 +286,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                        const __grid_constant__ PagedParams p, const PagedSplit out) {
   using S = PagedShape<D, FEW>;
   constexpr int SLABS = D / 64, TILE = S::TILE, RING = S::RING, SLAB = 128 * 128, QROWS = S::QROWS, QSLAB = QROWS * 128, Q_BYTES = S::Q_BYTES;
-  constexpr int NS = S::NS;
   constexpr uint32_t P_COL = S::P_COL, O_COL = S::O_COL;
   constexpr uint32_t IDESC_QK = make_idesc_bf16(128, 128, 0, 0), IDESC_PV = make_idesc_bf16(128, D, 0, 1);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *q_smem = smem + S::Q_AT, *ring = smem + S::RING_AT;      // (an MMA reads 128 rows: what follows stands in for missing ones)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS_AT);
-  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_free = bars + 8;      // scores are there [chain], have been loaded [S]
+  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_free = bars + 8;      // scores are there [chain], have been loaded
   uint64_t *p_ready = bars + 12, *o_done = bars + 14, *o_free = bars + 16, *few_done = bars + 17, *y_bar = bars + 18;      // y_bar: sums of the two chains are there [quarter]
   uint64_t *full = bars + 26, *empty = full + 2 * RING;      // up to 12 each
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
@@ -307,7 +311,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   // The copying warp sets up the barriers and goes on; the others meet it at a barrier that it only arrives at.
   if (warp == 9) {
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); }
+      for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); mbar_init(&s_full[i], 1); }
+      mbar_init(s_free, 4);
       for (int i = 0; i < 4; ++i) mbar_init(&y_bar[i], 2);
       mbar_init(o_free, FEW ? 1 : PA_SOFTMAX);
       mbar_init(few_done, 2);
@@ -331,7 +336,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     asm volatile("bar.sync 3, %0;" ::"n"(PA_THREADS) : "memory");
   }
   tc_fence_after();
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, warp == 9 ? 0u : *tmem_slot, 0);      // (warp 9 may be ahead of it)  S of chain t at 128 (t % NS), P at P_COL + 64 t, O at O_COL + D t
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, warp == 9 ? 0u : *tmem_slot, 0);      // (warp 9 may be ahead of it)  S at 0, P of chain t at P_COL + 64 t, O at O_COL + D t
   pdl_wait();
   if (warp == 10) pdl_trigger();              // after the TMEM allocation (see common.cuh): one thread's is the block's
   if (!FEW && threadIdx.x == 0) out.cut[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes what is cut, too)
@@ -433,7 +438,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // beside the operands that the tensor pipe reads from shared memory, and with ten waits and 32 MMAs for two tiles and a page one
     // warp took 5700 cycles, more than the softmax.  One warp for each chain would not see every phase of the barriers that it waits for.)
     bool ok = true;
-    int page = 0, q_done = 0, uses[2] = {0, 0};      // pages, items with keys, uses of a chain's S (NS = 1: of both's)
+    int page = 0, q_done = 0, tiles = 0;                // pages, items with keys, tiles of scores
     for (int k = 0; ok; ++k) {
       const Piece* at = piece_at(k);
       if (!at) break;
@@ -452,20 +457,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (pair ? g >= n[t] : (g & 1) != t) continue;
-          const int sb = NS == 1 ? 0 : t;
           const uint64_t qdesc = uniform_desc(smem_u32(q_smem + (qb + (pair ? t : 0)) * Q_BYTES), 16), kdesc = uniform_desc(smem_u32(ring + slot * TILE), 16);
-          if (uses[sb] > 0 && !(ok = wait_soon(&s_free[sb], (uint32_t)((uses[sb] - 1) & 1), 340))) break;      // what was in it has been loaded
+          if (tiles > 0 && !(ok = wait_soon(s_free, (uint32_t)((tiles - 1) & 1), 340))) break;      // the scores before have been loaded
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_ss(tmem_base + (uint32_t)(sb * 128), qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
+              umma_ss(tmem_base, qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
                       k != 0 ? 1u : 0u);
             umma_commit(&s_full[t]);
           }
           __syncwarp();
           if (!ok) break;
-          ++uses[sb];
+          ++tiles;
         }
         if (!ok) break;
         if (elect_one()) {
@@ -600,7 +604,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFTMAX_REGS));
     const int t = warp >> 2, q = warp & 3, row = q * 32 + lane;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)(t % NS * 128), p_addr = lane_addr + P_COL + (uint32_t)(t * 64), o_addr = lane_addr + O_COL + (uint32_t)(t * D);
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), p_addr = lane_addr + P_COL + (uint32_t)(t * 64), o_addr = lane_addr + O_COL + (uint32_t)(t * D);
     const int row_token = row / group;
     int done = 0, pieces = 0, turns[2] = {0, 0}, y_turn = 0;
     bool ok = true;
@@ -642,13 +646,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_after();
         if (active) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r + c * 32);
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32(lane_addr + c * 32, r + c * 32);
         }
         if (!handed) hand_over();
         if (active) tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[NS == 1 ? 0 : t]);
+        if (lane == 0) mbar_arrive(s_free);
         float alpha = 1.f;
         bool rescale = false;
         float neg_m = 0.f;
