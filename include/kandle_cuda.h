@@ -426,26 +426,32 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
  * tokens in one call (no counterpart in the reference, whose cache is contiguous and whose causal mask begins at position 0;
  * per sequence it is `scaled_dot_product_attention` of the last rows of a causal mask, packages/model-utils/src/attention/gqa.ts:407-414).
  *   q, out       bf16 [tokens,Hq,D] (D 64 or 128; strides multiples of 8), Hq a multiple (up to 64 times) of Hkv.  out must not be q
+ *   scale        between 1e-6 and 1e6
  *   k_pool, v_pool  bf16 [pages,Hkv,128,D]; block_table int32 [B,max_pages] (rows of any stride): entries behind a sequence's last
  *                page are not read
  *   ctx_len      int32 [B], or one number for all: the keys of sequence b, its new tokens' included (they are the last ones)
  *   q_start      int32 [B+1]: sequence b's new tokens are rows q_start[b] .. q_start[b+1] of q; rows outside stay as they are in out.
  *                NULL: tokens / B each
- *   max_query    the most new tokens of a sequence (0: not known, taken as `tokens`); a smaller bound makes fewer blocks
+ *   max_query    the most new tokens of a sequence (0: not known, taken as `tokens`); up to 32 / (Hq / Hkv) takes a form for
+ *                few rows
  * Token i of n sees positions 0 .. ctx_len - n + i; one that sees none gets a zero row.  Rows of a page behind a sequence's last key
  * may hold anything.  What the device tensors say is kept inside the buffers and reported at the next synchronisation: code 102 (more keys
- * than the table's pages), 103 (a page outside the pools, read as zeros), 104 (rows outside q, or more than max_query). */
+ * than the table's pages), 103 (a page outside the pools, read as zeros), 104 (rows outside q, or more than max_query).  Sums of parts
+ * of a sequence stand in the library's scratch (up to 60 MB, whatever the sizes): make the first call before a capture. */
 int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const kd_tensor* v_pool, const kd_tensor* block_table,
                        const kd_tensor* ctx_len, const kd_tensor* q_start, int max_query, float scale, const kd_tensor* out);
 /* Copies page src[i] to page dst[i] in every pool (each [pages,Hkv,128,D] of any type, all alike; the 128 rows of a head side by side):
  * a prefix for a sequence that will write on, or pages moved together.  src, dst int32 [n <= 65536].  A pair whose dst is in the lists
- * again is left out and reported (code 105), and one with a page outside the pools (103). */
+ * again is left out and reported (code 105), and one with a page outside the pools (103).  Lists of more than 4096 pairs use the
+ * library's scratch. */
 int kd_kv_pages_copy(const kd_tensor* const* pools, int n_pools, const kd_tensor* src, const kd_tensor* dst);
 /* Beams go on behind their parents.  parents int32 [requests,beams <= 32] (a beam's number within its request), block_table int32
  * [requests*beams,max_pages], spare int32 [requests*beams] (a page of its own for every beam, in no table), length one int32: the
  * positions that the beams hold.  Row r of the table receives the whole pages of its parent's row by reference.  The partly filled page
  * of a parent stays with its first child; the other children's rows get copies of its filled rows in their spare pages, and the last
- * pages of beams without children are the spare pages from then on.  Columns behind the held positions stay as they are. */
+ * pages of beams without children are the spare pages from then on.  Columns behind the held positions stay as they are.  A parent that
+ * is no beam of the request is taken as the beam itself and reported (code 106), as are a length beyond the table (102) and pages outside the
+ * pools (103).  Uses the library's scratch. */
 int kd_kv_pages_fork(const kd_tensor* const* pools, int n_pools, const kd_tensor* parents, const kd_tensor* block_table, const kd_tensor* spare,
                      const kd_tensor* length);
 /* A step of beam search: logits fp32 [requests,beams,V] or [requests*beams,V] (evenly spaced rows), scores fp32 [requests,beams <= 32].
@@ -453,7 +459,8 @@ int kd_kv_pages_fork(const kd_tensor* const* pools, int n_pools, const kd_tensor
  * finite is worth minus infinity.  The best `beams` candidates whose token is not eos (negative: none), best first: out_scores fp32 (may
  * be scores), parents int32 (their beam), tokens int64.  ended fp32 (or NULL): the value of (j, eos) where that is among the best
  * `beams` of all candidates, else minus infinity.  Candidates of one beam are ordered by their logits; equal ones go by the lower
- * beam, then the lower token. */
+ * beam, then the lower token; where there are fewer candidates, the rest are minus infinity with beam and token 0.  Uses the library's
+ * scratch. */
 int kd_beam_select(const kd_tensor* logits, const kd_tensor* scores, int eos, const kd_tensor* out_scores, const kd_tensor* parents,
                    const kd_tensor* tokens, const kd_tensor* ended);
 

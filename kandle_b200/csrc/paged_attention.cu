@@ -64,7 +64,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
 constexpr int PA_ROWS = 128;            // rows of a tile
 constexpr int PA_SOFTMAX = 8;           // warps 0-7: chain warp / 4, rows 32 (warp % 4) and on
 constexpr int PA_THREADS = 384;
-constexpr int PA_CACHE = 64;            // sequences whose lengths are kept in shared memory
+constexpr int PA_CACHE = 256;           // sequences whose lengths are kept in shared memory
 constexpr int PA_PIECES = 4;            // pieces of work that the warps of a block may be apart
 
 __device__ __forceinline__ float pa_exp2(float x) {
@@ -94,32 +94,31 @@ __device__ __forceinline__ void pa_add2(float& s0, float& s1, float a0, float a1
 }
 
 // ----------------------------------------------------------------------------- the division of the work
-// A sequence as an item of work sees it.  `units`: of all its items (0: no new tokens); a page of an item with two tiles counts twice, its two
-// softmaxes take twice as long.
-struct SeqWork {
-  int row0, n, ctx, units;
-};
 struct ItemShape {
   int group, tokens;                  // query heads on a KV head, tokens of a tile
-  __device__ __forceinline__ bool pair(int n) const { return n * group > PA_ROWS; }
-  __device__ __forceinline__ int items(int n) const { return pair(n) ? (n + 2 * tokens - 1) / (2 * tokens) : 1; }
-  // pages that an item's tokens see, and its units (one at least: tokens without keys get zero rows)
-  __device__ __forceinline__ int pages(const SeqWork& s, int item) const {
+  __device__ __forceinline__ bool pair(int n) const { return (int64_t)n * group > PA_ROWS; }
+  __device__ __forceinline__ int items(int n) const { return n == 0 ? 0 : pair(n) ? (n + 2 * tokens - 1) / (2 * tokens) : 1; }
+  // Pages that an item's tokens see, and its units: a page of an item with two tiles counts twice, its two softmaxes take twice as long (and one
+  // at least: tokens without keys get zero rows).
+  __device__ __forceinline__ int pages(const PagedSeq& s, int item) const {
     const int upto = pair(s.n) ? min(s.n, (item + 1) * 2 * tokens) : s.n;
     return (max(0, s.ctx - s.n + upto) + 127) / 128;
   }
-  __device__ __forceinline__ int units(const SeqWork& s, int item) const { return max(1, pages(s, item)) * (pair(s.n) ? 2 : 1); }
+  __device__ __forceinline__ int units(const PagedSeq& s, int item) const { return max(1, pages(s, item)) * (pair(s.n) ? 2 : 1); }
+  __device__ __forceinline__ int64_t all_units(const PagedSeq& s) const {
+    int64_t sum = 0;
+    for (int i = 0; i < items(s.n); ++i) sum += units(s, i);
+    return sum;
+  }
 };
-__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, const ItemShape& shape, int b) {
-  const PagedSeq q = paged_seq(p, b);
-  SeqWork s{q.row0, q.n, q.ctx, 0};
-  if (q.n > 0)
-    for (int i = 0; i < shape.items(q.n); ++i) s.units += shape.units(s, i);
-  return s;
-}
+struct CachedSeq {
+  PagedSeq s;
+  int64_t units;
+};
+__device__ __forceinline__ PagedSeq seq_of(const PagedParams& p, const CachedSeq* cache, int b) { return b < PA_CACHE ? cache[b].s : paged_seq(p, b); }
 // A block's piece of an item: pages j0 .. j0 + nb - 1.
 struct Piece {
-  SeqWork s;
+  PagedSeq s;
   int b, hk, item, j0, nb;
   int parts, part, first;             // parts of the whole item, this one's number, the block of the first one
   bool pair;
@@ -140,14 +139,13 @@ struct Walk {
   int64_t u, end, per;
   int b, hk, item, off, block;
   __device__ __forceinline__ int quotient(int64_t x) const { return (x | per) >> 32 ? (int)(x / per) : (int)((uint32_t)x / (uint32_t)per); }
-  __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape& shape, const int4* cache, Piece& w) {
+  __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape& shape, const CachedSeq* cache, Piece& w) {
     if (u >= end) return false;
     for (;;) {
       if (b == p.B) { b = 0; ++hk; }
       if (hk == p.Hkv) return false;
-      if (b < PA_CACHE) { const int4 c = cache[b]; w.s = SeqWork{c.x, c.y, c.z, c.w}; }
-      else w.s = seq_work(p, shape, b);
-      if (w.s.units && item < shape.items(w.s.n)) break;
+      w.s = seq_of(p, cache, b);
+      if (item < shape.items(w.s.n)) break;
       ++b;
       item = 0;
     }
@@ -168,13 +166,14 @@ struct Walk {
   }
 };
 // Block x's share, by one warp.
-__device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape& shape, int x, int blocks, int4* cache) {
+__device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape& shape, int x, int blocks, CachedSeq* cache) {
   const int lane = threadIdx.x & 31;
   int64_t sum = 0;
   for (int b = lane; b < p.B; b += 32) {
-    const SeqWork s = seq_work(p, shape, b);
-    if (b < PA_CACHE) cache[b] = make_int4(s.row0, s.n, s.ctx, s.units);
-    sum += s.units;
+    const PagedSeq s = paged_seq(p, b);
+    const int64_t n = shape.all_units(s);
+    if (b < PA_CACHE) cache[b] = CachedSeq{s, n};
+    sum += n;
   }
   __syncwarp();
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -190,7 +189,7 @@ __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape
   int64_t left = w.u - w.hk * sum;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b >= p.B ? 0 : b < PA_CACHE ? cache[b].w : seq_work(p, shape, b).units;
+    const int64_t n = b >= p.B ? 0 : b < PA_CACHE ? cache[b].units : shape.all_units(paged_seq(p, b));
     int64_t upto = n;
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -205,9 +204,7 @@ __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
-  SeqWork s;
-  if (w.b < PA_CACHE) { const int4 c = cache[w.b]; s = SeqWork{c.x, c.y, c.z, c.w}; }
-  else s = seq_work(p, shape, w.b);
+  const PagedSeq s = seq_of(p, cache, w.b);
   for (; left >= shape.units(s, w.item); ++w.item) left -= shape.units(s, w.item);
   w.off = (int)left;
   return w;
@@ -267,7 +264,7 @@ struct PagedShape {
   static constexpr int TILE = 128 * D * 2, RING = (FEW ? 3 : 2) * 32768 / TILE;      // slots for keys, and as many for values
   static constexpr int QROWS = FEW ? 32 : PA_ROWS, Q_BYTES = QROWS * D * 2;
   static constexpr int Q_AT = 0, RING_AT = 2 * Q_BYTES, BARS_AT = RING_AT + 2 * RING * TILE;
-  static constexpr int CACHE_AT = BARS_AT + 1024, ML_AT = CACHE_AT + PA_CACHE * 16, BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
+  static constexpr int CACHE_AT = BARS_AT + 1024, ML_AT = CACHE_AT + PA_CACHE * (int)sizeof(CachedSeq), BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
   // tensor memory: scores, probabilities, sums
   // (One buffer for the scores of both chains.  With heads of 64 there is room for two; the chains' softmaxes then run side by side, both at their
   // exponentials and both not, and a step takes 4400 cycles in place of 4000: 73.8 us against 71.2 in a batch of 12 x 700 tokens.)
@@ -302,7 +299,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   Piece* piece_s = reinterpret_cast<Piece*>(piece_empty + PA_PIECES);             // what the warps work on; no parts: behind the last one
   Piece* join_s = piece_s + PA_PIECES;                                            // [2]
   static_assert((52 + 2 * PA_PIECES) * 8 + (PA_PIECES + 2) * sizeof(Piece) <= 1024, "barriers and what stands behind them");
-  int4* cache = reinterpret_cast<int4*>(smem + S::CACHE_AT);
+  CachedSeq* cache = reinterpret_cast<CachedSeq*>(smem + S::CACHE_AT);
   float2* ml = reinterpret_cast<float2*>(smem + S::ML_AT);     // [piece & 1][chain][row] (maximum, sum)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const ItemShape shape{p.Hq / p.Hkv, QROWS / (p.Hq / p.Hkv)};
@@ -366,7 +363,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   // went through vector registers for every MMA and took 85 cycles each, whatever its size.
   auto uniform_desc = [](uint32_t addr, uint32_t lbo) { return make_smem_desc_sw128(__shfl_sync(0xffffffffu, addr, 0), lbo, 1024); };
   // where the outputs of a tile's row go
-  auto out_row = [&](const SeqWork& s, int hk, int token, int r) { return p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h; };
+  auto out_row = [&](const PagedSeq& s, int hk, int token, int r) { return p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h; };
 
   if (warp >= PA_SOFTMAX) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER_REGS));
@@ -967,6 +964,7 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   if (q_start) KD_TRY(tensor_ptr(q_start, &ps));
   KD_REQUIRE(((reinterpret_cast<uintptr_t>(pq) | reinterpret_cast<uintptr_t>(pk) | reinterpret_cast<uintptr_t>(pv) | reinterpret_cast<uintptr_t>(po)) & 15) == 0,
              "q, pools and out must be 16-byte aligned");
+  KD_REQUIRE(po != pq, "out must not be q");
   p.q = static_cast<const __nv_bfloat16*>(pq); p.k = static_cast<const __nv_bfloat16*>(pk); p.v = static_cast<const __nv_bfloat16*>(pv);
   p.o = static_cast<__nv_bfloat16*>(po);
   p.table = static_cast<const int*>(pt); p.ctx = static_cast<const int*>(pc); p.q_start = static_cast<const int*>(ps);

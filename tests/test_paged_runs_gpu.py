@@ -1,0 +1,177 @@
+"""Calls over a paged cache at the edges of what they take, and a step of beam search as a program makes it: the choice, the pages behind it and
+the attention over them in one captured graph."""
+import ctypes
+import json
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from kandle_b200 import core, io, lib, paged, synth
+from kandle_b200.core import Tensor
+from kandle_b200.model_utils import beam_select
+from tests.paged_cases import PAGE, attention_case, beam_answer, bf16, fork_answer
+from tests.test_beams_engine_gpu import DIMS, engine
+from tests.test_paged_gpu import check, put, run
+
+pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("count,most", [(300, 1), (700, 2), (260, 40)])
+def test_more_sequences_than_a_block_keeps(backend, count, most):
+    rng = np.random.default_rng(count)
+    new = rng.integers(0, most + 1, count).tolist()
+    new[-1] = most
+    c = attention_case(new, [n + int(k) for n, k in zip(new, rng.integers(0, 200, count))], 4, 2, 64, seed=count)
+    got = run(c, max_query=most)
+    check(c, got)
+    assert np.array_equal(run(c, max_query=most), got)
+
+
+@pytest.mark.parametrize("new,keys,heads,kv_heads,dim", [([301], [700], 64, 1, 64), ([131, 2], [131, 900], 96, 2, 128), ([1, 260], [40, 290], 43, 1, 64)])
+def test_tiles_of_few_tokens(backend, new, keys, heads, kv_heads, dim):
+    """Groups of 64, 48 and 43 heads: two tokens to a tile, and rows of it that nobody has."""
+    c = attention_case(new, keys, heads, kv_heads, dim, seed=heads)
+    check(c, run(c))
+
+
+def test_outputs_in_place_of_the_queries_are_refused(backend):
+    c = attention_case([2], [5], 4, 2, 64)
+    q = put(c["q"])
+    with pytest.raises(lib.KandleCudaError) as e:
+        paged.attention(q, put(c["k"]), put(c["v"]), put(c["table"]), put(c["keys"]), put(c["start"]), out=q)
+    assert e.value.status == 1
+
+
+@pytest.mark.parametrize("n", [1000, 4096, 4097, 6000])
+def test_long_lists_of_copies(backend, n):
+    rng = np.random.default_rng(n)
+    order = rng.permutation(2 * n + 5).astype(np.int32)
+    values = [rng.integers(-128, 128, (2 * n + 5, 1, PAGE, 8)).astype(np.float32) for _ in range(2)]
+    pools = [Tensor(v, dtype="bfloat16") for v in values]
+    src, dst = order[:n].copy(), order[n:2 * n].copy()
+    paged.copy_pages(pools, Tensor(src), Tensor(dst))
+    backend.synchronize()
+    for v, p in zip(values, pools):
+        v[dst] = v[src]
+        assert np.array_equal(p.dataAsync(), v)
+    # the last pair goes where the first does, and one in the middle to where another comes from
+    dst[-1], dst[n // 2] = dst[0], src[n // 3]
+    left_out = [0, n - 1, n // 2]
+    src[:] = rng.permutation(src)
+    if src[n // 2] == dst[n // 2]:
+        src[[n // 2, 1]] = src[[1, n // 2]]
+    paged.copy_pages(pools, Tensor(src), Tensor(dst))
+    with pytest.raises(lib.KandleCudaError, match="error code 105"):
+        backend.synchronize()
+    good = np.setdiff1d(np.arange(n), left_out)
+    for v, p in zip(values, pools):
+        v[dst[good]] = v[src[good]]
+        assert np.array_equal(p.dataAsync(), v)
+
+
+class Step:
+    """beams of two requests over one layer's cache, on the host and on the device."""
+
+    def __init__(self, length, seed, B=2, K=3, V=5000, heads=8, kv_heads=4, dim=64):
+        rng = np.random.default_rng(seed)
+        R, width = B * K, -(-max(length, 1) // PAGE) + 1
+        pages = R * width + R
+        order = rng.permutation(pages)
+        self.table = order[:R * width].reshape(B, K, width).astype(np.int32)
+        self.table[:, :, :length // PAGE] = self.table[:, :1, :length // PAGE]
+        self.table = self.table.reshape(R, width)
+        self.spare = order[R * width:].astype(np.int32)
+        self.pools = [bf16(rng.standard_normal((pages, kv_heads, PAGE, dim))).float().numpy() for _ in range(2)]
+        self.q = bf16(rng.standard_normal((R, heads, dim)) * 1.5)
+        self.logits = (rng.standard_normal((B, K, V)) * 2.5).astype(np.float32)
+        self.scores = (-3 * rng.random((B, K))).astype(np.float32)
+        self.length, self.eos = length, 17
+
+    def put(self):
+        d = {n: Tensor(getattr(self, n)) for n in ("table", "spare", "logits", "scores")}
+        d["q"], d["length"] = put(self.q), Tensor(np.array([self.length], np.int32))
+        d["pools"] = [Tensor(p, dtype="bfloat16") for p in self.pools]
+        d["out"] = core.empty(tuple(self.q.shape), "bfloat16")
+        d["choice"] = beam_select(d["logits"], d["scores"], self.eos)
+        return d
+
+    def copy_to(self, d):
+        fresh = self.put()
+        for n in ("table", "spare", "logits", "scores", "q", "length"):
+            core.copy_(d[n], fresh[n])
+        for a, b in zip(d["pools"], fresh["pools"]):
+            core.copy_(a, b)
+
+    def call(self, d):
+        beam_select(d["logits"], d["scores"], self.eos, out=(d["scores"], *d["choice"][1:]))
+        paged.fork_pages(d["pools"], d["choice"][1], d["table"], d["spare"], d["length"])
+        paged.attention(d["q"], *d["pools"], d["table"], d["length"], max_query=1, out=d["out"])
+
+    def check(self, d):
+        scores, parents, tokens, _ = beam_answer(self.logits, self.scores, self.eos)
+        assert np.array_equal(d["choice"][1].dataAsync(), parents) and np.array_equal(d["choice"][2].dataAsync(), tokens)
+        assert (np.abs(d["scores"].dataAsync() - scores) <= 60 * 2.0 ** -24 + np.abs(scores) * 2.0 ** -24).all()
+        pools = [p.copy() for p in self.pools]
+        table, spare = fork_answer(pools, parents, self.table, self.spare, self.length)
+        assert np.array_equal(d["table"].dataAsync(), table) and np.array_equal(d["spare"].dataAsync(), spare)
+        assert all(np.array_equal(a.dataAsync(), b) for a, b in zip(d["pools"], pools))
+        R = len(table)
+        check({"q": self.q, "k": bf16(pools[0]), "v": bf16(pools[1]), "table": table, "start": np.arange(R + 1), "keys": np.full(R, self.length), "scale": self.q.shape[-1] ** -0.5},
+              d["out"].dataAsync())
+
+
+@pytest.mark.parametrize("pdl", [0, 1])
+def test_two_captured_steps_share_the_scratch(backend, pdl):
+    """Replayed in turn, between calls that are not captured; each on a cache of another length."""
+    first, second = Step(200, 1), Step(391, 2, B=1, K=8)
+    states, graphs = [first.put(), second.put()], []
+    for s, d in zip((first, second), states):
+        s.call(d)
+        s.check(d)
+    for s, d in zip((first, second), states):
+        lib.call("kd_graph_begin")
+        lib.call("kd_set_pdl", pdl)
+        try:
+            s.call(d)
+        finally:
+            lib.call("kd_set_pdl", 0)
+        g = ctypes.c_uint64(0)
+        lib.call("kd_graph_end", ctypes.byref(g))
+        graphs.append(g)
+    loose = attention_case([3, 200], [300, 450], 8, 4, 64)
+    for seed in (3, 4, 5):
+        news = [Step(130 + 9 * seed, seed), Step(385 + seed, 10 * seed, B=1, K=8)]
+        for s, d in zip(news, states):
+            s.copy_to(d)
+        lib.call("kd_graph_launch", graphs[0])
+        lib.call("kd_graph_launch", graphs[1])
+        check(loose, run(loose))
+        for s, d in zip(news, states):
+            s.check(d)
+    for g in graphs:
+        lib.call("kd_graph_destroy", g)
+
+
+def test_command_line_searches_with_beams(backend, tmp_path):
+    w = {k: lib.round_to_bf16(v) for k, v in synth.qwen3_weights(std=0.05, head_dim=64, **DIMS).items()}
+    (tmp_path / "config.json").write_text(json.dumps({"architectures": ["Qwen3ForCausalLM"], "vocab_size": 1024, "hidden_size": 256, "intermediate_size": 512, "num_hidden_layers": 3,
+                                                      "num_attention_heads": 4, "num_key_value_heads": 2, "head_dim": 64}))
+    io.save_file({k: (lib.f32_to_bf16_bits(v).reshape(np.shape(v)), "BF16") for k, v in w.items()}, str(tmp_path / "model.safetensors"))
+    ids = synth.token_ids("cli.beams", (2, 30), 1024)
+    command = [sys.executable, "-m", "kandle_b200.generate", "--model", str(tmp_path), "--steps", "5", "--beams", "3", "--eos", "9"]
+    for row in ids:
+        command += ["--prompt", " ".join(map(str, row))]
+    r = subprocess.run(command, capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert r.returncode == 0, r.stderr[-2000:]
+    eng = engine(64, batch=6, room=35, paged=True, spare_pages=12)
+    want = [h[0][0] for h in eng.generate_beams(ids, 3, 5, 9)]
+    eng.dispose()
+    assert [[int(x) for x in line.split()] for line in r.stdout.strip().split("\n")] == want
+    for more in (["--temperature", "0.5"], ["--beams", "-1"]):
+        r = subprocess.run(command + more, capture_output=True, text=True, timeout=300, cwd=ROOT)
+        assert r.returncode == 2 and "--beams" in r.stderr
