@@ -436,8 +436,9 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
  *                few rows
  * Token i of n sees positions 0 .. ctx_len - n + i; one that sees none gets a zero row.  Rows of a page behind a sequence's last key
  * may hold anything.  What the device tensors say is kept inside the buffers and reported at the next synchronisation: code 102 (more keys
- * than the table's pages), 103 (a page outside the pools, read as zeros), 104 (rows outside q, or more than max_query).  Sums of parts
- * of a sequence stand in the library's scratch (up to 60 MB, whatever the sizes): make the first call before a capture. */
+ * than the table's pages), 103 (a page outside the pools, read as zeros), 104 (rows outside q, or more than max_query),
+ * 107 (2^31 pages or more, times Hkv and the tiles of 128 rows that go through them: nothing is done).  Sums of parts of a sequence stand in the
+ * library's scratch (up to 60 MB, whatever the sizes): make the first call before a capture. */
 int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const kd_tensor* v_pool, const kd_tensor* block_table,
                        const kd_tensor* ctx_len, const kd_tensor* q_start, int max_query, float scale, const kd_tensor* out);
 /* Copies page src[i] to page dst[i] in every pool (each [pages,Hkv,128,D] of any type, all alike; the 128 rows of a head side by side):

@@ -94,20 +94,22 @@ __device__ __forceinline__ void pa_add2(float& s0, float& s1, float a0, float a1
 }
 
 // ----------------------------------------------------------------------------- the division of the work
+// One warp goes through all of this while the others wait for it, an instruction after the other: it has no division but where an item is cut.
+template <bool FEW>
 struct ItemShape {
   int group, tokens;                  // query heads on a KV head, tokens of a tile
-  __device__ __forceinline__ bool pair(int n) const { return (int64_t)n * group > PA_ROWS; }
-  __device__ __forceinline__ int items(int n) const { return n == 0 ? 0 : pair(n) ? (n + 2 * tokens - 1) / (2 * tokens) : 1; }
+  __device__ __forceinline__ bool pair(int n) const { return !FEW && n > tokens; }
+  __device__ __forceinline__ bool has(int n, int item) const { return pair(n) ? item * 2 * tokens < n : item < min(n, 1); }
   // Pages that an item's tokens see, and its units: a page of an item with two tiles counts twice, its two softmaxes take twice as long (and one
   // at least: tokens without keys get zero rows).
   __device__ __forceinline__ int pages(const PagedSeq& s, int item) const {
     const int upto = pair(s.n) ? min(s.n, (item + 1) * 2 * tokens) : s.n;
-    return (max(0, s.ctx - s.n + upto) + 127) / 128;
+    return (max(0, s.ctx - s.n + upto) + 127) >> 7;
   }
-  __device__ __forceinline__ int units(const PagedSeq& s, int item) const { return max(1, pages(s, item)) * (pair(s.n) ? 2 : 1); }
+  __device__ __forceinline__ int units(const PagedSeq& s, int item) const { return max(1, pages(s, item)) << (pair(s.n) ? 1 : 0); }
   __device__ __forceinline__ int64_t all_units(const PagedSeq& s) const {
     int64_t sum = 0;
-    for (int i = 0; i < items(s.n); ++i) sum += units(s, i);
+    for (int i = 0; has(s.n, i); ++i) sum += units(s, i);
     return sum;
   }
 };
@@ -123,7 +125,8 @@ struct Piece {
   int parts, part, first;             // parts of the whole item, this one's number, the block of the first one
   bool pair;
   // pages of the two chains
-  __device__ __forceinline__ void tiles(const ItemShape& shape, int (&n)[2]) const {
+  template <bool FEW>
+  __device__ __forceinline__ void tiles(const ItemShape<FEW>& shape, int (&n)[2]) const {
     n[0] = (nb + 1) / 2;
     n[1] = nb / 2;
     if (!pair) return;
@@ -134,30 +137,30 @@ struct Piece {
     }
   }
 };
-// Goes through the pieces of a block.
+// Goes through the pieces of a block: units u .. end - 1 of a row of fewer than 2^31, `per` a block.
 struct Walk {
-  int64_t u, end, per;
+  unsigned u, end, per;
   int b, hk, item, off, block;
-  __device__ __forceinline__ int quotient(int64_t x) const { return (x | per) >> 32 ? (int)(x / per) : (int)((uint32_t)x / (uint32_t)per); }
-  __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape& shape, const CachedSeq* cache, Piece& w) {
+  template <bool FEW>
+  __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape<FEW>& shape, const CachedSeq* cache, Piece& w) {
     if (u >= end) return false;
     for (;;) {
       if (b == p.B) { b = 0; ++hk; }
       if (hk == p.Hkv) return false;
       w.s = seq_of(p, cache, b);
-      if (item < shape.items(w.s.n)) break;
+      if (shape.has(w.s.n, item)) break;
       ++b;
       item = 0;
     }
     w.pair = shape.pair(w.s.n);
-    const int all = shape.units(w.s, item), pages = shape.pages(w.s, item), weight = w.pair ? 2 : 1;
-    const int take = (int)min((int64_t)(all - off), end - u);
-    const int64_t start = u - off;
+    const int pages = shape.pages(w.s, item), twice = w.pair ? 1 : 0, all = max(1, pages) << twice;
+    const int take = min(all - off, (int)(end - u));
+    const unsigned start = u - off;
     w.b = b; w.hk = hk; w.item = item;
-    w.j0 = min(off / weight, pages);
-    w.nb = min((off + take) / weight, pages) - w.j0;
-    w.first = off ? quotient(start) : block;
-    w.parts = (start + all <= end ? block : quotient(start + all - 1)) - w.first + 1;
+    w.j0 = min(off >> twice, pages);
+    w.nb = min((off + take) >> twice, pages) - w.j0;
+    w.first = off ? (int)(start / per) : block;
+    w.parts = (start + all <= end ? block : (int)((start + all - 1) / per)) - w.first + 1;
     w.part = block - w.first;
     u += take;
     off = 0;
@@ -166,33 +169,42 @@ struct Walk {
   }
 };
 // Block x's share, by one warp.
-__device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape& shape, int x, int blocks, CachedSeq* cache) {
+template <bool FEW>
+__device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape<FEW>& shape, int x, int blocks, CachedSeq* cache) {
   const int lane = threadIdx.x & 31;
-  int64_t sum = 0;
+  uint64_t own = 0;
   for (int b = lane; b < p.B; b += 32) {
     const PagedSeq s = paged_seq(p, b);
     const int64_t n = shape.all_units(s);
     if (b < PA_CACHE) cache[b] = CachedSeq{s, n};
-    sum += n;
+    own += n;
   }
   __syncwarp();
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const int64_t all = sum * p.Hkv;
+  own = min(own, (uint64_t)1 << 42);
+  const uint64_t sum64 = ((uint64_t)__reduce_add_sync(0xffffffffu, (unsigned)(own >> 16)) << 16) + __reduce_add_sync(0xffffffffu, (unsigned)(own & 0xffff));
   Walk w;
-  w.per = max((int64_t)1, (all + blocks - 1) / blocks);
-  w.u = min(all, x * w.per);
-  w.end = min(all, w.u + w.per);
+  w.u = w.end = 0;
+  w.per = 1;
   w.hk = w.b = w.item = w.off = 0;
   w.block = x;
+  if (sum64 * p.Hkv >= 0x80000000u) {
+    if (lane == 0 && atomicCAS(p.err, 0, 107) == 0) { p.err[1] = (int)(sum64 >> 31); p.err[2] = (int)(sum64 & 0x7fffffff); }
+    return w;
+  }
+  const unsigned sum = (unsigned)sum64, all = sum * p.Hkv;
+  w.per = max(1u, (all + blocks - 1) / blocks);
+  w.u = (unsigned)min((uint64_t)all, (uint64_t)x * w.per);
+  w.end = min(all, w.u + w.per);
   if (w.u >= w.end) return w;
   w.hk = (int)(w.u / sum);
-  int64_t left = w.u - w.hk * sum;
+  unsigned left = w.u - w.hk * sum;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    const int64_t n = b >= p.B ? 0 : b < PA_CACHE ? cache[b].units : shape.all_units(paged_seq(p, b));
-    int64_t upto = n;
+    const unsigned n = b >= p.B ? 0u : (unsigned)(b < PA_CACHE ? cache[b].units : shape.all_units(paged_seq(p, b)));
+    unsigned upto = n;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, upto > left);
@@ -205,7 +217,7 @@ __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
   const PagedSeq s = seq_of(p, cache, w.b);
-  for (; left >= shape.units(s, w.item); ++w.item) left -= shape.units(s, w.item);
+  for (; left >= (unsigned)shape.units(s, w.item); ++w.item) left -= shape.units(s, w.item);
   w.off = (int)left;
   return w;
 }
@@ -302,7 +314,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   CachedSeq* cache = reinterpret_cast<CachedSeq*>(smem + S::CACHE_AT);
   float2* ml = reinterpret_cast<float2*>(smem + S::ML_AT);     // [piece & 1][chain][row] (maximum, sum)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const ItemShape shape{p.Hq / p.Hkv, QROWS / (p.Hq / p.Hkv)};
+  const ItemShape<FEW> shape{p.Hq / p.Hkv, QROWS / (p.Hq / p.Hkv)};
   const int group = shape.group;
 
   // The copying warp sets up the barriers and goes on; the others meet it at a barrier that it only arrives at.
@@ -856,7 +868,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   pdl_trigger();
   const int4 c = in.cut[blockIdx.x];
   if (c.w <= 1) return;
-  const ItemShape shape{p.Hq / p.Hkv, PA_ROWS / (p.Hq / p.Hkv)};
+  const ItemShape<false> shape{p.Hq / p.Hkv, PA_ROWS / (p.Hq / p.Hkv)};
   const PagedSeq s = paged_seq(p, c.x);
   const bool pair = shape.pair(s.n);
   for (int n = threadIdx.x; n < 32 * (D / 4); n += 256) {

@@ -47,6 +47,21 @@ def test_outputs_in_place_of_the_queries_are_refused(backend):
     assert e.value.status == 1
 
 
+def test_more_pages_than_are_counted_are_refused(backend):
+    """2048 sequences that all name the same 2^20 pages: reported, and nothing is read or written."""
+    B, pages = 2048, 1 << 20
+    pool = core.zeros((2, 1, PAGE, 64), "bfloat16")
+    table = core.zeros((1, pages), "int32").expand([B, pages])
+    out = core.full((B, 2, 64), 7.0, "bfloat16")
+    q = core.zeros((B, 2, 64), "bfloat16")
+    paged.attention(q, pool, pool, table, core.full((1,), pages * PAGE, "int32"), out=out)
+    with pytest.raises(lib.KandleCudaError, match="error code 107"):
+        backend.synchronize()
+    assert (out.dataAsync() == 7.0).all()
+    ones = core.full((1,), 1, "int32")
+    assert (paged.attention(q, pool, pool, table, ones, out=out).dataAsync() == 0.0).all()
+
+
 @pytest.mark.parametrize("n", [1000, 4096, 4097, 6000])
 def test_long_lists_of_copies(backend, n):
     rng = np.random.default_rng(n)
