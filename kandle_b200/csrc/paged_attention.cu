@@ -11,8 +11,8 @@
 //
 // Division.  The pages of all items of all KV heads stand in one row, and each of as many persistent blocks as SMs takes an equal share of it, from
 // wherever it begins in one item to wherever it ends in another: long and short sequences, prompts and single tokens load every SM
-// alike.  An item that is cut leaves unnormalised sums that are joined, by the block that is through last where they are small (up to
-// 32 rows), else by a second kernel.
+// alike.  An item that is cut leaves unnormalised sums, which are joined by the block that is through last if they are of one tile, else by a
+// second kernel.
 //
 // Softmax.  A thread owns a row and loads its 128 scores at once; S is free from then on, so that the next Q K^T runs beside the exponentials
 // (with P over S it waited for P V, and a chain's step was the sum of both: 4331 cycles for two tiles and a page, of which the exponential unit
@@ -227,7 +227,7 @@ __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape
 struct PagedSplit {
   float* part_o;      // [place][rows][D] unnormalised sums, or [place][D / 4][rows][4] of items with two tiles
   float2* part_ml;    // [place][rows] (running maximum in the log2 domain, sum)
-  int4* cut;          // what began in block x and went on: (sequence, KV head, item, parts)
+  int4* cut;          // what of two tiles began in block x and went on: (sequence, KV head, item, parts)
 };
 // Parts of a cut item that are through, by its first block; the last one sets it back.
 constexpr int PA_BLOCKS = 1024;
@@ -238,12 +238,6 @@ static __device__ unsigned g_paged_through[PA_BLOCKS];
 // 57.5 us with rows side by side, 53.5 so).
 template <int D>
 __device__ __forceinline__ int part_at(bool pair, int r, int c) { return pair ? c / 4 * (2 * PA_ROWS) + r : r * (D / 4) + c / 4; }
-// The n-th row and four channels of an item to join, in the same order.
-template <int D>
-__device__ __forceinline__ void part_nth(bool pair, int n, int& r, int& c) {
-  r = pair ? n / (2 * D) * 8 + n % 8 : n / (D / 4);
-  c = pair ? n % (2 * D) / 8 * 4 : n % (D / 4) * 4;
-}
 // Four channels of a row from all parts of an item: sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
 template <int D>
 __device__ __forceinline__ void join_parts(const PagedSplit& in, int part_rows, bool pair, int r, int c, int first, int parts, __nv_bfloat16* to) {
@@ -370,6 +364,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   auto piece_done = [&](int k) {
     __syncwarp();
     if (lane == 0) mbar_arrive(&piece_empty[k % PA_PIECES]);
+  };
+  // A warp's part of a cut item is written.  The last of all its parts' warps leaves the item to be joined at the end of its block (in the parts'
+  // order, whoever is last).
+  auto part_through = [&](const Piece& w, int warps) {
+    unsigned before;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(&g_paged_through[w.first]) : "memory");
+    if (before == (unsigned)(w.parts * warps) - 1) {
+      g_paged_through[w.first] = 0;
+      join_s[atomicAdd(joins, 1)] = w;
+    }
   };
   // Descriptors and addresses pass through a shuffle, which tells the compiler that they are alike in a warp: what was made of numbers read from memory
   // went through vector registers for every MMA and took 85 cycles each, whatever its size.
@@ -597,16 +601,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (real && !direct) out.part_ml[at] = make_float2(M, L);
       __syncwarp();
       if (w.nb > 0) ++pieces;
-      if (!direct && lane == 0) {
-        // the part that is through last joins them all, at the end of its block (in the parts' order, whoever is last)
-        unsigned before;
-        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(&g_paged_through[w.first]) : "memory");
-        if (before == (unsigned)w.parts - 1) {
-          g_paged_through[w.first] = 0;
-          join_s[*joins] = w;
-          ++*joins;
-        }
-      }
+      if (!direct && lane == 0) part_through(w, 1);
       __syncwarp();
     }
   }
@@ -762,7 +757,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       const bool direct = w.parts == 1;
       const int place = 2 * blockIdx.x + (w.part == 0 ? 1 : 0);
-      if (threadIdx.x == 0 && !direct && w.part == 0) out.cut[blockIdx.x] = make_int4(w.b, w.hk, w.item, w.parts);
+      if (threadIdx.x == 0 && pair && !direct && w.part == 0) out.cut[blockIdx.x] = make_int4(w.b, w.hk, w.item, w.parts);
       // the chains' shares of an output; where both worked on the same rows, each needs the other's statistics
       float f[2] = {0.f, 0.f}, M = m, L = l;
       if (w.nb > 0 && active) {
@@ -824,6 +819,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         if (real && !direct && (pair || t == 0)) out.part_ml[(int64_t)place * (2 * PA_ROWS) + part_row] = make_float2(M, L);
       }
+      if (!pair && !direct) {
+        __syncwarp();
+        if (lane == 0) part_through(w, PA_SOFTMAX);
+      }
       piece_done(k);
       if (!some) continue;
       // (nobody counts twice in a phase: the piece before is over)
@@ -843,13 +842,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       for (int v = 0; v < 2; ++v)
         for (int i = max(0, issued[v] - RING); i < issued[v]; ++i) landed(&full[v * RING + i % RING], i / RING);
     }
-  } else if (FEW) {
+  } else {
     for (int i = 0; i < *joins; ++i) {
       const Piece& j = join_s[i];
       for (int n = threadIdx.x; n < j.s.n * group * (D / 4); n += PA_THREADS) {
-        int r, c;
-        part_nth<D>(false, n, r, c);
-        join_parts<D>(out, QROWS, false, r, c, j.first, j.parts, out_row(j.s, j.hk, r / group, r));
+        const int r = n / (D / 4);
+        join_parts<D>(out, FEW ? QROWS : 2 * PA_ROWS, false, r, n % (D / 4) * 4, j.first, j.parts, out_row(j.s, j.hk, r / group, r));
       }
     }
   }
@@ -860,24 +858,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   }
 }
 
-// Items of the kernel above that were cut and have more than 32 rows: block (x, y) has 32 rows of what began in block x and went on, four channels
-// a thread.
+// Items of two tiles that were cut by the kernel above: block (x, y) has 32 rows of what began in block x and went on, four channels a thread.
+// (By one block, 256 rows of four to five parts would take as long as the launch.)
 template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p, const PagedSplit in) {
   pdl_wait();
   pdl_trigger();
   const int4 c = in.cut[blockIdx.x];
   if (c.w <= 1) return;
-  const ItemShape<false> shape{p.Hq / p.Hkv, PA_ROWS / (p.Hq / p.Hkv)};
+  const int group = p.Hq / p.Hkv, tokens = PA_ROWS / group;
   const PagedSeq s = paged_seq(p, c.x);
-  const bool pair = shape.pair(s.n);
   for (int n = threadIdx.x; n < 32 * (D / 4); n += 256) {
-    int r, ch;
-    part_nth<D>(pair, n, r, ch);
-    r += blockIdx.y * 32;
-    const int i = (pair ? (2 * c.z + r / PA_ROWS) * shape.tokens : 0) + r % PA_ROWS / shape.group;
-    if (r % PA_ROWS >= shape.tokens * shape.group || i >= s.n || (!pair && r >= PA_ROWS)) continue;
-    join_parts<D>(in, 2 * PA_ROWS, pair, r, ch, blockIdx.x, c.w, p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)(c.y * shape.group + r % PA_ROWS % shape.group) * p.so_h);
+    const int r = blockIdx.y * 32 + n / (2 * D) * 8 + n % 8, i = (2 * c.z + r / PA_ROWS) * tokens + r % PA_ROWS / group;      // (eight rows side by side)
+    if (r % PA_ROWS >= tokens * group || i >= s.n) continue;
+    join_parts<D>(in, 2 * PA_ROWS, true, r, n % (2 * D) / 8 * 4, blockIdx.x, c.w, p.o + (int64_t)(s.row0 + i) * p.so_t + (int64_t)(c.y * group + r % PA_ROWS % group) * p.so_h);
   }
 }
 
@@ -914,7 +908,7 @@ static int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const Page
   out.cut = reinterpret_cast<int4*>(out.part_ml + places);
   KD_CUDA_CHECK(launch_ex(paged_attention_kernel<D, FEW>, dim3(blocks), dim3(PA_THREADS), (size_t)S::SMEM, tq, tk, tv, p, out));
   KD_TRY(after_launch("paged_attention_kernel"));
-  if constexpr (!FEW) {
+  if ((int64_t)p.max_query * group > PA_ROWS) {
     KD_CUDA_CHECK(launch_behind(paged_join_kernel<D>, dim3(blocks, 2 * PA_ROWS / 32), dim3(256), 0, p, out));
     KD_TRY(after_launch("paged_join_kernel"));
   }
