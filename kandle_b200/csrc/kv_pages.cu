@@ -1,7 +1,8 @@
 // Pages of a cache: copies to other places (kd_kv_pages_copy) and beams that take over their parents' pages (kd_kv_pages_fork).
 //
 // A pool is [pages,Hkv,128,D] with rows of a head side by side; a call works on all pools of a model at once (keys and values of every
-// layer), whose addresses travel in the launch's parameters.  Bound: HBM, every moved byte read and written once.
+// layer), whose addresses travel in the launch's parameters.  Bound: HBM, every moved byte read and written once: 300 pages of 18 pools (2.8 GB moved) 428 us, 6.6
+// TB/s; 16 requests of 8 beams at 1000 positions 80 us, 6.1 TB/s.  Two pages 14 us, four beams 15 us: the launches.
 #include "common.cuh"
 #include "kernels.cuh"
 

@@ -19,9 +19,9 @@
 // needs 2048 and the tensor pipe 2048).  Tensor memory holds one S for both chains, which they use in turn, two P and two O.  Two threads a
 // row (and 16 warps) were slower: they have to exchange the maximum.
 //
-// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 85 us, 4.45 TB/s, of which some 25 are the launch, the division,
-// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8) 54 us; 4 x 2048 tokens on 6144 (32 on 8) 1007 us, 955
-// TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
+// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 84 us, 4.5 TB/s, of which some 25 are the launch, the division,
+// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 47 us; 4 x 2048 tokens on 6144 (32 on 8) 997 us,
+// 965 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
 #include "common.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
@@ -273,7 +273,7 @@ struct PagedShape {
   static constexpr int CACHE_AT = BARS_AT + 1024, ML_AT = CACHE_AT + PA_CACHE * (int)sizeof(CachedSeq), BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
   // tensor memory: scores, probabilities, sums
   // (One buffer for the scores of both chains.  With heads of 64 there is room for two; the chains' softmaxes then run side by side, both at their
-  // exponentials and both not, and a step takes 4400 cycles in place of 4000: 73.8 us against 71.2 in a batch of 12 x 700 tokens.)
+  // exponentials and both not, and a step takes 4400 cycles in place of 4000: 73.8 us against 71.0 in a batch of 12 x 700 tokens.)
   static constexpr uint32_t P_COL = 128, O_COL = P_COL + 128;
   static_assert(O_COL + 2 * D <= 512, "tensor memory has 512 columns");
   // registers of a thread of warps 8-11 and of the others: the outputs' warp needs its own, else the scores do
