@@ -11,7 +11,7 @@
 //
 // Division.  The pages of all items of all KV heads stand in one row, and each of as many persistent blocks as SMs takes an equal share of it, from
 // wherever it begins in one item to wherever it ends in another: long and short sequences, prompts and single tokens load every SM
-// alike.  An item that is cut leaves unnormalised sums, which are joined by the block that is through last if they are of one tile, else by a
+// alike.  (Where items are few, whole items or equal pieces of them: paged_walk.)  An item that is cut leaves unnormalised sums, which are joined by the block that is through last if they are of one tile, else by a
 // second kernel.
 //
 // Softmax.  A thread owns a row and loads its 128 scores at once; S is free from then on, so that the next Q K^T runs beside the exponentials
@@ -20,8 +20,8 @@
 // row (and 16 warps) were slower: they have to exchange the maximum.
 //
 // Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 84 us, 4.5 TB/s, of which some 25 are the launch, the division,
-// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 47 us; 4 x 2048 tokens on 6144 (32 on 8) 997 us,
-// 965 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
+// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 45 us; 4 x 2048 tokens on 6144 (32 on 8) 1005 us,
+// 960 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
 #include "common.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
@@ -94,7 +94,7 @@ __device__ __forceinline__ void pa_add2(float& s0, float& s1, float a0, float a1
 }
 
 // ----------------------------------------------------------------------------- the division of the work
-// One warp goes through all of this while the others wait for it, an instruction after the other: it has no division but where an item is cut.
+// One warp goes through all of this while the others wait for it, an instruction after the other, and so with few divisions.
 template <bool FEW>
 struct ItemShape {
   int group, tokens;                  // query heads on a KV head, tokens of a tile
@@ -107,9 +107,37 @@ struct ItemShape {
     return (max(0, s.ctx - s.n + upto) + 127) >> 7;
   }
   __device__ __forceinline__ int units(const PagedSeq& s, int item) const { return max(1, pages(s, item)) << (pair(s.n) ? 1 : 0); }
-  __device__ __forceinline__ int64_t all_units(const PagedSeq& s) const {
+  __device__ __forceinline__ int64_t all_units(const PagedSeq& s, int& items, int& most) const {
     int64_t sum = 0;
-    for (int i = 0; has(s.n, i); ++i) sum += units(s, i);
+    for (int i = 0; has(s.n, i); ++i) {
+      const int u = units(s, i);
+      sum += u;
+      most = max(most, u);
+      ++items;
+    }
+    return sum;
+  }
+};
+// Items in equal pieces of at most `per` units (whole pages).
+struct Pieces {
+  unsigned most[2];                   // pages of a piece of one tile and of two
+  uint64_t by[2];                     // 2^32 divided by them, rounded up: quotients of numbers up to 2^16 are exact
+  __device__ __forceinline__ explicit Pieces(unsigned per) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      most[i] = max(1u, per >> i);
+      by[i] = (uint64_t)(0xffffffffu / most[i]) + 1;
+    }
+  }
+  template <bool FEW>
+  __device__ __forceinline__ int of(const ItemShape<FEW>& shape, const PagedSeq& s, int item) const {
+    const bool pair = shape.pair(s.n);
+    return (int)(((max(1, shape.pages(s, item)) + (pair ? most[1] : most[0]) - 1) * (pair ? by[1] : by[0])) >> 32);
+  }
+  template <bool FEW>
+  __device__ __forceinline__ int all(const ItemShape<FEW>& shape, const PagedSeq& s) const {
+    int sum = 0;
+    for (int i = 0; shape.has(s.n, i); ++i) sum += of(shape, s, i);
     return sum;
   }
 };
@@ -137,10 +165,11 @@ struct Piece {
     }
   }
 };
-// Goes through the pieces of a block: units u .. end - 1 of a row of fewer than 2^31, `per` a block.
+// Goes through the pieces of a block: units u .. end - 1 of a row of fewer than 2^31, `per` a block; or the one piece `part` of `parts` that begins
+// at `off` of its item and has up to `end` units.
 struct Walk {
   unsigned u, end, per;
-  int b, hk, item, off, block;
+  int b, hk, item, off, block, parts, part;
   template <bool FEW>
   __device__ __forceinline__ bool next(const PagedParams& p, const ItemShape<FEW>& shape, const CachedSeq* cache, Piece& w) {
     if (u >= end) return false;
@@ -159,66 +188,119 @@ struct Walk {
     w.b = b; w.hk = hk; w.item = item;
     w.j0 = min(off >> twice, pages);
     w.nb = min((off + take) >> twice, pages) - w.j0;
-    w.first = off ? (int)(start / per) : block;
-    w.parts = (start + all <= end ? block : (int)((start + all - 1) / per)) - w.first + 1;
+    if (parts) {
+      w.first = block - part;
+      w.parts = parts;
+      u = end;
+    } else {
+      w.first = off ? (int)(start / per) : block;
+      w.parts = (start + all <= end ? block : (int)((start + all - 1) / per)) - w.first + 1;
+      u += take;
+    }
     w.part = block - w.first;
-    u += take;
     off = 0;
     ++item;
     return true;
   }
 };
-// Block x's share, by one warp.
+// A cut in units: what the partial sums and the join of an item cost beside a page, with few rows and with more; and what a second item costs a block.
+constexpr unsigned PA_CUT_FEW = 2, PA_CUT = 10, PA_SECOND = 4;
+
+// Block x's share, by one warp: an equal share of all units, wherever that cuts an item; or, where there are no more items than blocks, an item or
+// an equal piece of one, if the longest share is then longer by no more than what a cut or a second item costs (8 KV heads of 128, in a graph: 16 single
+// tokens on 1000 positions 22.8 us in equal shares, 18.8 as whole items; 30 tokens on 900 29.3 and 21.7; 4 x 200 on 600 36.6 and 24.9; one token
+// on 700, which is cut either way, 12.9 and 13.4: the choice itself).
 template <bool FEW>
 __device__ __forceinline__ Walk paged_walk(const PagedParams& p, const ItemShape<FEW>& shape, int x, int blocks, CachedSeq* cache) {
+  constexpr unsigned ALL = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   uint64_t own = 0;
+  int items = 0, most = 0;
   for (int b = lane; b < p.B; b += 32) {
     const PagedSeq s = paged_seq(p, b);
-    const int64_t n = shape.all_units(s);
+    const int64_t n = shape.all_units(s, items, most);
     if (b < PA_CACHE) cache[b] = CachedSeq{s, n};
     own += n;
   }
   __syncwarp();
   own = min(own, (uint64_t)1 << 42);
-  const uint64_t sum64 = ((uint64_t)__reduce_add_sync(0xffffffffu, (unsigned)(own >> 16)) << 16) + __reduce_add_sync(0xffffffffu, (unsigned)(own & 0xffff));
+  items = min(items, 1 << 20);
+  const uint64_t sum64 = ((uint64_t)__reduce_add_sync(ALL, (unsigned)(own >> 16)) << 16) + __reduce_add_sync(ALL, (unsigned)(own & 0xffff));
   Walk w;
   w.u = w.end = 0;
   w.per = 1;
-  w.hk = w.b = w.item = w.off = 0;
+  w.hk = w.b = w.item = w.off = w.parts = w.part = 0;
   w.block = x;
   if (sum64 * p.Hkv >= 0x80000000u) {
     if (lane == 0 && atomicCAS(p.err, 0, 107) == 0) { p.err[1] = (int)(sum64 >> 31); p.err[2] = (int)(sum64 & 0x7fffffff); }
     return w;
   }
-  const unsigned sum = (unsigned)sum64, all = sum * p.Hkv;
+  unsigned sum = (unsigned)sum64;
+  const unsigned all = sum * p.Hkv;
   w.per = max(1u, (all + blocks - 1) / blocks);
-  w.u = (unsigned)min((uint64_t)all, (uint64_t)x * w.per);
-  w.end = min(all, w.u + w.per);
-  if (w.u >= w.end) return w;
-  w.hk = (int)(w.u / sum);
-  unsigned left = w.u - w.hk * sum;
+  unsigned one = 0;                                  // one piece a block, of up to so many units
+  const unsigned longest = __reduce_max_sync(ALL, most);
+  if ((uint64_t)__reduce_add_sync(ALL, items) * p.Hkv <= blocks && longest < 32768) {
+    // a lane tries one of up to eight lengths with a quarter of the sequences
+    const unsigned more = min((unsigned)lane & 7, PA_SECOND), per = longest <= w.per + more + (FEW ? PA_CUT_FEW : PA_CUT) ? longest : w.per + more;
+    const Pieces cut(per);
+    int n = 0;
+    for (int b = lane >> 3; b < p.B; b += 4) n += cut.all(shape, seq_of(p, cache, b));
+    n += __shfl_xor_sync(ALL, n, 8);
+    n += __shfl_xor_sync(ALL, n, 16);
+    const unsigned fits = __ballot_sync(ALL, n * p.Hkv <= blocks);
+    if (fits) {
+      one = __shfl_sync(ALL, per, __ffs(fits) - 1);
+      sum = __shfl_sync(ALL, n, __ffs(fits) - 1);
+    }
+  }
+  const Pieces cut(max(1u, one));
+  unsigned left;
+  if (one) {
+    if (x >= (int)(sum * p.Hkv)) return w;
+    left = x;
+  } else {
+    w.u = (unsigned)min((uint64_t)all, (uint64_t)x * w.per);
+    w.end = min(all, w.u + w.per);
+    if (w.u >= w.end) return w;
+    left = w.u;
+  }
+  w.hk = (int)(left / sum);
+  left -= w.hk * sum;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    const unsigned n = b >= p.B ? 0u : (unsigned)(b < PA_CACHE ? cache[b].units : shape.all_units(paged_seq(p, b)));
+    unsigned n = 0;
+    if (b < p.B) {
+      int i = 0, m = 0;
+      n = one ? cut.all(shape, seq_of(p, cache, b)) : (unsigned)(b < PA_CACHE ? cache[b].units : shape.all_units(paged_seq(p, b), i, m));
+    }
     unsigned upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+      const unsigned v = __shfl_up_sync(ALL, upto, o);
       if (lane >= o) upto += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, upto > left);
+    const unsigned hit = __ballot_sync(ALL, upto > left);
     if (hit) {
       const int who = __ffs(hit) - 1;
       w.b = b0 + who;
-      left -= __shfl_sync(0xffffffffu, upto - n, who);
+      left -= __shfl_sync(ALL, upto - n, who);
       break;
     }
-    left -= __shfl_sync(0xffffffffu, upto, 31);
+    left -= __shfl_sync(ALL, upto, 31);
   }
   const PagedSeq s = seq_of(p, cache, w.b);
-  for (; left >= (unsigned)shape.units(s, w.item); ++w.item) left -= shape.units(s, w.item);
-  w.off = (int)left;
+  if (!one) {
+    for (; left >= (unsigned)shape.units(s, w.item); ++w.item) left -= shape.units(s, w.item);
+    w.off = (int)left;
+    return w;
+  }
+  for (; left >= (unsigned)cut.of(shape, s, w.item); ++w.item) left -= cut.of(shape, s, w.item);
+  w.parts = cut.of(shape, s, w.item);
+  w.part = (int)left;
+  const int size = (max(1, shape.pages(s, w.item)) + w.parts - 1) / w.parts << (shape.pair(s.n) ? 1 : 0);
+  w.off = w.part * size;
+  w.end = size;
   return w;
 }
 
