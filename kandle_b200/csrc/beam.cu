@@ -421,7 +421,7 @@ KD_API int kd_beam_select(const kd_tensor* logits, const kd_tensor* scores, int 
   else
     KD_REQUIRE(logits->shape[0] == B * K, "logits must hold one row for each of %lld x %lld beams", (long long)B, (long long)K);
   KD_REQUIRE(logits->strides[last] == 1 || V == 1, "unit stride along the vocabulary required");
-  KD_REQUIRE(V >= 2 && V <= 0x7fffffff - 8192 && eos < V, "a vocabulary of at least two tokens, among them the end token (or a negative one for none), is required");
+  KD_REQUIRE(V >= 2 && V <= (1 << 30) && eos < V, "a vocabulary of 2 to 2^30 tokens, among them the end token (or a negative one for none), is required");
   KD_REQUIRE(B * K <= 65535, "%lld beams: up to 65535 a call", (long long)(B * K));
   KD_REQUIRE(out_scores->dtype == KD_F32 && is_contiguous(out_scores) && numel(out_scores) == B * K && parents->dtype == KD_I32 && is_contiguous(parents) &&
                  numel(parents) == B * K && tokens->dtype == KD_I64 && is_contiguous(tokens) && numel(tokens) == B * K,

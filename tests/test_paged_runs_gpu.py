@@ -172,6 +172,14 @@ def test_two_captured_steps_share_the_scratch(backend, pdl):
         lib.call("kd_graph_destroy", g)
 
 
+def test_vocabularies_beyond_two_to_the_30_are_refused(backend):
+    logits = core.empty((1, 1, (1 << 30) + 4), "float32")
+    with pytest.raises(lib.KandleCudaError) as e:
+        beam_select(logits, core.zeros((1, 1)), -1)
+    assert e.value.status == 1
+    logits.dispose()
+
+
 def test_command_line_searches_with_beams(backend, tmp_path):
     w = {k: lib.round_to_bf16(v) for k, v in synth.qwen3_weights(std=0.05, head_dim=64, **DIMS).items()}
     (tmp_path / "config.json").write_text(json.dumps({"architectures": ["Qwen3ForCausalLM"], "vocab_size": 1024, "hidden_size": 256, "intermediate_size": 512, "num_hidden_layers": 3,
