@@ -10,7 +10,7 @@
 // 4096 hardly any are.  The first bound: with q = 1, 2 or 4, the q-th largest of a warp's lanes' maxima, and of these the one
 // that ceil(K / q) of the eight warps reach, so at least K logits reach it.
 //
-// Bound: HBM, 4 bytes a logit, where there are many rows: 32 requests of 4 beams over 151936 tokens (78 MB) 29 us, of which the pass takes 17 (4.6
+// Bound: HBM, 4 bytes a logit, where there are many rows: 32 requests of 4 beams over 151936 tokens (78 MB) 28 us, of which the pass takes 16 (4.9
 // TB/s: four blocks an SM with 16 KB each on the way, which stop for the bound at their first step) and the join of a request 6, a chain of short
 // steps by one block; the rest is the launch.  One request of 4 beams 13.7 us, all latency: 2.4 of them the pass.  Two launches (lists, then the
 // join) took 110 and 20.5, with the lists ranked by every pair of a step.
@@ -98,10 +98,29 @@ struct BeamShared {
   BeamBest cand[BM_CAND], chosen[BM_BEAMS], ends[BM_BEAMS], top[8];
 };
 
-__device__ __forceinline__ float exp_of(float x) {
+__device__ __forceinline__ float exp2_of(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+constexpr float BM_LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * BM_LOG2E); }
+// exp(a - m) of two numbers, added to two sums.  (The difference first: a times log2 e may be beyond fp32 where masks are its
+// lowest number.  A fused multiply-add would save 1 us of 28 in the largest case.)
+__device__ __forceinline__ void add_exp(float& s0, float& s1, float a0, float a1, float minus_m) {
+  float x0, x1;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "add.rn.f32x2 d, a, c;\n\tmul.rn.f32x2 d, d, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(BM_LOG2E), "f"(minus_m));
+  x0 = exp2_of(x0);
+  x1 = exp2_of(x1);
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(s0), "+f"(s1) : "f"(x0), "f"(x1));
+}
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // The segments' lists of request b are there: its outputs.  By the whole block.  One block runs this once, out of a cold instruction cache: short
@@ -282,7 +301,7 @@ __global__ void __launch_bounds__(BM_THREADS, 4) beam_kernel(const BeamParams p)
     __syncthreads();
     return n;
   };
-  float r[BM_NE], ahead[BM_NE], m = -INFINITY, s = 0.f, bound = -INFINITY;
+  float r[BM_NE], ahead[BM_NE], m = -INFINITY, s = 0.f, s1 = 0.f, bound = -INFINITY;
   bool above = false;               // only logits above the bound count (else those that reach it)
   int kept = 0;
   if (t == 0) sh.count = 0;
@@ -292,22 +311,25 @@ __global__ void __launch_bounds__(BM_THREADS, 4) beam_kernel(const BeamParams p)
 #pragma unroll
     for (int e = 0; e < BM_NE; ++e) r[e] = ahead[e];
     if (base + BM_STEP < hi) load(base + BM_STEP, ahead);
-    float top = r[0];
+    float four[BM_NE / 4], top;
+    auto tops = [&]() {
 #pragma unroll
-    for (int e = 1; e < BM_NE; ++e) top = fmaxf(top, r[e]);
+      for (int e = 0; e < BM_NE; e += 4) four[e / 4] = fmaxf(max_of(r[e], r[e + 1], r[e + 2]), r[e + 3]);
+      top = fmaxf(max_of(four[0], four[1], four[2]), four[3]);
+    };
+    tops();
     // the thread's own maximum and sum; terms far below vanish, NaN and infinity stay
-    const float now = fmaxf(m, top), from = now == -INFINITY ? 0.f : now;
-    s *= exp_of(m - from);
+    const float now = fmaxf(m, top), from = now == -INFINITY ? 0.f : now, scale = exp_of(m - from);
+    s *= scale;
+    s1 *= scale;
     m = now;
 #pragma unroll
-    for (int e = 0; e < BM_NE; ++e) s += exp_of(r[e] - from);
+    for (int e = 0; e < BM_NE; e += 2) add_exp(s, s1, r[e], r[e + 1], -from);
     if (p.eos >= base && p.eos < base + BM_STEP) {
-      top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < BM_NE; ++e) {
+      for (int e = 0; e < BM_NE; ++e)
         if (index(base, e) == p.eos) r[e] = -INFINITY;
-        top = fmaxf(top, r[e]);
-      }
+      tops();
     }
     if (step == 0) {
       const float u = warp_nth(top, quota, -INFINITY);
@@ -317,11 +339,15 @@ __global__ void __launch_bounds__(BM_THREADS, 4) beam_kernel(const BeamParams p)
     }
     if (above ? top > bound : top >= bound) {
 #pragma unroll
-      for (int e = 0; e < BM_NE; ++e) {
-        const int i = index(base, e);
-        if ((above ? r[e] > bound : r[e] >= bound) && i < hi && i != p.eos) {
-          const int n = atomicAdd(&sh.count, 1);
-          if (n < BM_CAP) sh.keys[n] = beam_key(r[e], i);
+      for (int g = 0; g < BM_NE; g += 4) {
+        if (!(above ? four[g / 4] > bound : four[g / 4] >= bound)) continue;
+#pragma unroll
+        for (int e = g; e < g + 4; ++e) {
+          const int i = index(base, e);
+          if ((above ? r[e] > bound : r[e] >= bound) && i < hi && i != p.eos) {
+            const int n = atomicAdd(&sh.count, 1);
+            if (n < BM_CAP) sh.keys[n] = beam_key(r[e], i);
+          }
         }
       }
     }
@@ -370,7 +396,7 @@ __global__ void __launch_bounds__(BM_THREADS, 4) beam_kernel(const BeamParams p)
   }
   // the segment's maximum and sum
   const float all = warp_max(m), from = all == -INFINITY ? 0.f : all;
-  s = warp_sum(s * exp_of(m - from));
+  s = warp_sum((s + s1) * exp_of(m - from));
   if (lane == 0) sh.red[w] = make_float2(all, s);
   __syncthreads();
   const int64_t place = row * p.segs + blockIdx.x;

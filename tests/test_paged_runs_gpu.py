@@ -172,6 +172,20 @@ def test_two_captured_steps_share_the_scratch(backend, pdl):
         lib.call("kd_graph_destroy", g)
 
 
+@pytest.mark.parametrize("low", [-3.4028235e38, -2.5e38])
+def test_rows_of_the_lowest_numbers(backend, low):
+    """A beam whose mask leaves nothing is uniform over its tokens, as in float64; one that it leaves something has those."""
+    logits = np.full((1, 3, 9000), low, np.float32)
+    logits[0, 1, [5, 4100, 8999]] = [1.0, 3.0, 2.0]
+    logits[0, 2, ::2] = 0.25
+    scores = np.array([[-0.5, -1.0, -0.75]], np.float32)
+    s, p, t, e = (x.dataAsync() for x in beam_select(Tensor(logits), Tensor(scores), 4100))
+    want = beam_answer(logits, scores, 4100)
+    assert np.array_equal(p, want[1]) and np.array_equal(t, want[2])
+    # 9000 equal terms in fp32: each addition is off by half a step of the sum so far at most, in chains of 32, and the exponential by 2^-22
+    assert (np.abs(s - want[0]) <= 60 * 2.0 ** -24 + np.abs(want[0]) * 2.0 ** -24).all() and np.array_equal(np.isfinite(e), np.isfinite(want[3]))
+
+
 def test_vocabularies_beyond_two_to_the_30_are_refused(backend):
     logits = core.empty((1, 1, (1 << 30) + 4), "float32")
     with pytest.raises(lib.KandleCudaError) as e:
