@@ -427,8 +427,8 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
  * per sequence it is `scaled_dot_product_attention` of the last rows of a causal mask, packages/model-utils/src/attention/gqa.ts:407-414).
  *   q, out       bf16 [tokens,Hq,D] (D 64 or 128; strides multiples of 8), Hq a multiple (up to 64 times) of Hkv.  out must not be q
  *   scale        between 1e-6 and 1e6
- *   k_pool, v_pool  bf16 [pages,Hkv,128,D]; block_table int32 [B,max_pages] (rows of any stride): entries behind a sequence's last
- *                page are not read
+ *   k_pool, v_pool  bf16 [pages,Hkv,128,D]; block_table int32 [B <= 65535, max_pages <= 2^18] (rows of any stride): entries behind a
+ *                sequence's last page are not read
  *   ctx_len      int32 [B], or one number for all: the keys of sequence b, its new tokens' included (they are the last ones)
  *   q_start      int32 [B+1]: sequence b's new tokens are rows q_start[b] .. q_start[b+1] of q; rows outside stay as they are in out.
  *                NULL: tokens / B each

@@ -1028,7 +1028,8 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
     KD_REQUIRE(k_pool->strides[i] % 8 == 0 && v_pool->strides[i] % 8 == 0 && k_pool->strides[i] >= 0 && v_pool->strides[i] >= 0, "strides must be multiples of 8 elements");
   KD_REQUIRE(k_pool->shape[0] >= 1, "the pools hold no page");
   KD_REQUIRE(block_table->ndim == 2 && block_table->dtype == KD_I32 && block_table->strides[1] == 1 && block_table->strides[0] >= 0, "block_table must be int32 [B,max_pages] with rows in one piece");
-  KD_REQUIRE(block_table->shape[0] <= 65535 && block_table->shape[1] < (1 << 24), "the block table is too large");
+  // (a warp waits for all pages of a piece, at most 2 us each, and gives up after a second)
+  KD_REQUIRE(block_table->shape[0] <= 65535 && block_table->shape[1] <= (1 << 18), "the block table is too large: up to 65535 sequences of 2^18 pages are handled");
   const int B = (int)block_table->shape[0], max_pages = (int)block_table->shape[1];
   KD_REQUIRE(ctx_len->dtype == KD_I32 && is_contiguous(ctx_len) && (numel(ctx_len) == B || numel(ctx_len) == 1), "ctx_len must be int32 [B] or one number for all");
   KD_REQUIRE(scale >= 1e-6f && scale <= 1e6f, "scale must lie between 1e-6 and 1e6");

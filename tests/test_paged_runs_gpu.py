@@ -8,11 +8,12 @@ import sys
 
 import numpy as np
 import pytest
+import torch
 
 from kandle_b200 import core, io, lib, paged, synth
 from kandle_b200.core import Tensor
 from kandle_b200.model_utils import beam_select
-from tests.paged_cases import PAGE, attention_case, beam_answer, bf16, fork_answer
+from tests.paged_cases import PAGE, attention_answer, attention_case, beam_answer, bf16, fork_answer
 from tests.test_beams_engine_gpu import DIMS, engine
 from tests.test_paged_gpu import check, put, run
 
@@ -47,9 +48,20 @@ def test_outputs_in_place_of_the_queries_are_refused(backend):
     assert e.value.status == 1
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (64, 1, 64), (40, 1, 128)])
+def test_a_context_that_repeats_itself(backend, heads, kv_heads, dim):
+    """Five pages 1000 times over, 640000 positions: one token's answer is that of the five.  The sums are longer than attention_answer counts: chains of up to
+    34 pages of 128 keys a block in fp32, 2^-24 for an addition, so 2^-11 of the mass for the sum and as much for its divisor: a quarter of its 2^-8."""
+    c = attention_case([1], [5 * PAGE], heads, kv_heads, dim, seed=dim)
+    want, tol = attention_answer(c)
+    table = np.ascontiguousarray(np.tile(c["table"], (1, 1000)))
+    got = run(dict(c, table=table, keys=c["keys"] * 1000), max_query=1)
+    assert ((torch.tensor(got).double() - want).abs() <= 1.25 * tol).all()
+
+
 def test_more_pages_than_are_counted_are_refused(backend):
-    """2048 sequences that all name the same 2^20 pages: reported, and nothing is read or written."""
-    B, pages = 2048, 1 << 20
+    """8192 sequences that all name the same 2^18 pages: reported, and nothing is read or written."""
+    B, pages = 8192, 1 << 18
     pool = core.zeros((2, 1, PAGE, 64), "bfloat16")
     table = core.zeros((1, pages), "int32").expand([B, pages])
     out = core.full((B, 2, 64), 7.0, "bfloat16")
@@ -59,6 +71,9 @@ def test_more_pages_than_are_counted_are_refused(backend):
         backend.synchronize()
     assert (out.dataAsync() == 7.0).all()
     ones = core.full((1,), 1, "int32")
+    with pytest.raises(lib.KandleCudaError) as e:
+        paged.attention(q, pool, pool, core.zeros((1, pages + 1), "int32").expand([B, pages + 1]), ones, out=out)
+    assert e.value.status == 1
     assert (paged.attention(q, pool, pool, table, ones, out=out).dataAsync() == 0.0).all()
 
 
