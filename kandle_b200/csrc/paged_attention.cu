@@ -17,10 +17,11 @@
 // Softmax.  A thread owns a row and loads its 128 scores at once; S is free from then on, so that the next Q K^T runs beside the exponentials
 // (with P over S it waited for P V, and a chain's step was the sum of both: 4331 cycles for two tiles and a page, of which the exponential unit
 // needs 2048 and the tensor pipe 2048).  Tensor memory holds one S for both chains, which they use in turn, two P and two O.  Two threads a
-// row (and 16 warps) were slower: they have to exchange the maximum.
+// row (and 16 warps) were slower: they have to exchange the maximum.  With up to 32 rows (FEW) one warp has a tile, and its instructions have to come
+// for it alone: short loops over 32 scores at a time, P over S.
 //
-// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 84 us, 4.5 TB/s, of which some 25 are the launch, the division,
-// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 45 us; 4 x 2048 tokens on 6144 (32 on 8) 1005 us,
+// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 80 us, 4.7 TB/s, of which some 20 are the launch, the division,
+// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 44 us; 4 x 2048 tokens on 6144 (32 on 8) 1000 us,
 // 960 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
 #include "common.cuh"
 #include "kernels.cuh"
@@ -354,12 +355,13 @@ struct PagedShape {
   static constexpr int Q_AT = 0, RING_AT = 2 * Q_BYTES, BARS_AT = RING_AT + 2 * RING * TILE;
   static constexpr int CACHE_AT = BARS_AT + 1024, ML_AT = CACHE_AT + PA_CACHE * (int)sizeof(CachedSeq), BYTES = ML_AT + 2 * 2 * PA_ROWS * 8;
   // tensor memory: scores, probabilities, sums
-  // (One buffer for the scores of both chains.  With heads of 64 there is room for two; the chains' softmaxes then run side by side, both at their
-  // exponentials and both not, and a step takes 4400 cycles in place of 4000: 73.8 us against 71.0 in a batch of 12 x 700 tokens.)
-  static constexpr uint32_t P_COL = 128, O_COL = P_COL + 128;
+  // (FEW: scores of each chain, with the probabilities over them.  Else one buffer for the scores of both chains.  With heads of 64 there is room
+  // for two; the chains' softmaxes then run side by side, both at their exponentials and both not, and a step takes 4400 cycles in place of
+  // 4000: 73.8 us against 71.0 in a batch of 12 x 700 tokens.)
+  static constexpr uint32_t S_STEP = FEW ? 128 : 0, P_COL = FEW ? 0 : 128, P_STEP = FEW ? 128 : 64, O_COL = 256;
   static_assert(O_COL + 2 * D <= 512, "tensor memory has 512 columns");
-  // registers of a thread of warps 8-11 and of the others: the outputs' warp needs its own, else the scores do
-  static constexpr int OTHER_REGS = FEW ? 120 : 72, SOFTMAX_REGS = FEW ? 192 : 216;
+  // registers of a thread of warps 8-11 and of the others, which hold 128 scores (FEW: 32, and all have what they were launched with)
+  static constexpr int OTHER_REGS = 72, SOFTMAX_REGS = 216;
   static_assert((PA_THREADS - PA_SOFTMAX * 32) * OTHER_REGS + PA_SOFTMAX * 32 * SOFTMAX_REGS <= PA_THREADS * 168, "registers of the launch");
   static constexpr int SMEM = BYTES + 1024;
   static_assert(SMEM <= 227 * 1024, "tiles exceed shared memory");
@@ -371,7 +373,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                        const __grid_constant__ PagedParams p, const PagedSplit out) {
   using S = PagedShape<D, FEW>;
   constexpr int SLABS = D / 64, TILE = S::TILE, RING = S::RING, SLAB = 128 * 128, QROWS = S::QROWS, QSLAB = QROWS * 128, Q_BYTES = S::Q_BYTES;
-  constexpr uint32_t P_COL = S::P_COL, O_COL = S::O_COL;
+  constexpr uint32_t S_STEP = S::S_STEP, P_COL = S::P_COL, P_STEP = S::P_STEP, O_COL = S::O_COL;
   constexpr uint32_t IDESC_QK = make_idesc_bf16(128, 128, 0, 0), IDESC_PV = make_idesc_bf16(128, D, 0, 1);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -464,7 +466,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   auto out_row = [&](const PagedSeq& s, int hk, int token, int r) { return p.o + (int64_t)(s.row0 + token) * p.so_t + (int64_t)(hk * group + r % group) * p.so_h; };
 
   if (warp >= PA_SOFTMAX) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER_REGS));
+  if constexpr (!FEW) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER_REGS));
   if (warp == 9) {
     // This warp alone goes through the division: its state does not fit beside the others' registers, and each began a piece some 4000 cycles late.
     Walk walk = paged_walk(p, shape, blockIdx.x, gridDim.x, cache);
@@ -533,7 +535,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // beside the operands that the tensor pipe reads from shared memory, and with ten waits and 32 MMAs for two tiles and a page one
     // warp took 5700 cycles, more than the softmax.  One warp for each chain would not see every phase of the barriers that it waits for.)
     bool ok = true;
-    int page = 0, q_done = 0, tiles = 0;                // pages, items with keys, tiles of scores
+    int page = 0, q_done = 0, tiles[2] = {0, 0};                // pages, items with keys, tiles of scores
     for (int k = 0; ok; ++k) {
       const Piece* at = piece_at(k);
       if (!at) break;
@@ -553,18 +555,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         for (int t = 0; t < 2; ++t) {
           if (pair ? g >= n[t] : (g & 1) != t) continue;
           const uint64_t qdesc = uniform_desc(smem_u32(q_smem + (qb + (pair ? t : 0)) * Q_BYTES), 16), kdesc = uniform_desc(smem_u32(ring + slot * TILE), 16);
-          if (tiles > 0 && !(ok = wait_soon(s_free, (uint32_t)((tiles - 1) & 1), 340))) break;      // the scores before have been loaded
+          // the scores before have been loaded (FEW: and the probabilities in their place used)
+          if (FEW) ok = tiles[t] == 0 || wait_soon(&o_done[t], (uint32_t)((tiles[t] - 1) & 1), 340);
+          else ok = tiles[0] == 0 || wait_soon(s_free, (uint32_t)((tiles[0] - 1) & 1), 340);
+          if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_ss(tmem_base, qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
+              umma_ss(tmem_base + (uint32_t)t * S_STEP, qdesc + ((uint32_t)((k / 4) * QSLAB + (k % 4) * 32) >> 4), kdesc + ((uint32_t)((k / 4) * SLAB + (k % 4) * 32) >> 4), IDESC_QK,
                       k != 0 ? 1u : 0u);
             umma_commit(&s_full[t]);
           }
           __syncwarp();
           if (!ok) break;
-          ++tiles;
+          ++tiles[FEW ? t : 0];
         }
         if (!ok) break;
         if (elect_one()) {
@@ -604,7 +609,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              umma_ts(tmem_base + O_COL + (uint32_t)(t * D), tmem_base + P_COL + (uint32_t)(t * 64 + k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV, k != 0 ? 1u : more);
+              umma_ts(tmem_base + O_COL + (uint32_t)(t * D), tmem_base + P_COL + (uint32_t)t * P_STEP + (uint32_t)(k * 8), vdesc + (uint32_t)(k * 128), IDESC_PV, k != 0 ? 1u : more);
             umma_commit(&o_done[t]);
           }
           __syncwarp();
@@ -688,9 +693,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFTMAX_REGS));
+    if constexpr (!FEW) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFTMAX_REGS));
     const int t = warp >> 2, q = warp & 3, row = q * 32 + lane;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), p_addr = lane_addr + P_COL + (uint32_t)(t * 64), o_addr = lane_addr + O_COL + (uint32_t)(t * D);
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)t * S_STEP, p_addr = lane_addr + P_COL + (uint32_t)t * P_STEP, o_addr = lane_addr + O_COL + (uint32_t)(t * D);
     const int row_token = row / group;
     int done = 0, pieces = 0, turns[2] = {0, 0}, y_turn = 0;
     bool ok = true;
@@ -718,10 +723,103 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       };
       for (int i = 0; i < mine; ++i, ++my_turn) {
         const int g = pair ? i : 2 * i + t, kv0 = (w.j0 + g) * 128;
-        uint32_t r[128];
-        float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f;
         const bool masked = kv0 + 127 > hidden;                     // some row does not see all of these keys
         const int lim = last - kv0;
+        float mx0 = -1e30f, mx1 = -1e30f, mx2 = -1e30f, mx3 = -1e30f, alpha = 1.f, neg_m = 0.f, sum0 = 0.f, sum1 = 0.f;
+        bool rescale = false;
+        // The maximum is raised only when it grew by more than 2^8: the sum uses the same one, so nothing is lost.
+        auto raise = [&] {
+          const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * p.scale_log2;
+          if (i == 0 || !real) {                                    // (nobody reads a padding row)
+            m = m_blk;
+          } else if (m_blk - m > 8.0f) {
+            alpha = pa_exp2(m - m_blk);
+            m = m_blk;
+            rescale = true;
+          }
+          neg_m = -m;
+        };
+        auto rescale_sums = [&] {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {                     // narrow pieces: the scores stay in registers meanwhile
+            uint32_t o[16];
+            tmem_ld_32x16(o_addr + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st_32x16(o_addr + c, o);
+          }
+          l *= alpha;
+        };
+        // Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them (by
+        // the chain whose product comes first).
+        auto clear_values = [&] {
+          // (what stood in the slot before has been used, so that the parity is that of this page)
+          if (i == 0 && pieces > 0 && !wait(o_free, (uint32_t)((pieces - 1) & 1), 333)) return false;
+          const int slot = RING + (done + g) % RING;
+          if (!wait(&full[slot], (uint32_t)(((done + g) / RING) & 1), 330)) return false;
+          if (kv0 + row >= w.s.ctx) {
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d) *reinterpret_cast<uint4*>(ring + slot * TILE + (d / 8) * SLAB + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_proxy();
+          return true;
+        };
+        const bool unclean = kv0 + 128 > w.s.ctx && (!pair || t == 0 || i >= n[0]);
+        if constexpr (FEW) {
+          // One warp works on a tile here, and straight code for 128 scores comes to it at a few cycles an instruction (5300 a tile, with eight warps 3300):
+          // short loops over 32 scores, which are read twice.  S of this chain is overwritten by P, and its next Q K^T waits for P V.
+          if (!(ok = wait(&s_full[t], (uint32_t)(my_turn & 1), 329))) break;
+          tc_fence_after();
+          if (active) {
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t r[32];
+              tmem_ld_32x32(s_addr + c, r);
+              tmem_wait_ld();
+              if (masked) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (e > lim - c) r[e] = __float_as_uint(-1e30f);
+              }
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                mx0 = pa_max3(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+                mx1 = pa_max3(mx1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+                mx2 = pa_max3(mx2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
+                mx3 = pa_max3(mx3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
+              }
+            }
+            raise();
+            if (__any_sync(0xffffffffu, rescale)) rescale_sums();      // (the product before is complete, or there were no scores)
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t r[32];
+              tmem_ld_32x32(s_addr + c, r);
+              tmem_wait_ld();
+              if (masked) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (e > lim - c) r[e] = __float_as_uint(-1e30f);
+              }
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float x0, x1;
+                pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), p.scale_log2, neg_m);
+                const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
+                pa_add2(sum0, sum1, e0, e1);
+                r[e] = pack_bf16(e0, e1);
+              }
+              tmem_st_32x16(p_addr + c / 2, r);
+            }
+          }
+          if (unclean && !(ok = clear_values())) break;
+          hand_over();
+          l += sum0 + sum1;
+          continue;
+        }
+        uint32_t r[128];
         // P of the tile before is handed over when its store is done: while the scores are waited for, or else behind their load
         bool handed = i == 0;
         if (!handed && !__all_sync(0xffffffffu, mbar_test(&s_full[t], (uint32_t)(my_turn & 1)))) {
@@ -732,16 +830,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_after();
         if (active) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32(lane_addr + c * 32, r + c * 32);
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r + c * 32);
         }
         if (!handed) hand_over();
         if (active) tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
-        float alpha = 1.f;
-        bool rescale = false;
-        float neg_m = 0.f;
         if (active) {
           if (masked) {
 #pragma unroll
@@ -755,20 +850,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             mx2 = pa_max3(mx2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
             mx3 = pa_max3(mx3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
           }
-          const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * p.scale_log2;
-          // The maximum is raised only when it grew by more than 2^8: the sum uses the same one, so nothing is lost.
-          if (i == 0 || !real) {                                    // (nobody reads a padding row)
-            m = m_blk;
-          } else if (m_blk - m > 8.0f) {
-            alpha = pa_exp2(m - m_blk);
-            m = m_blk;
-            rescale = true;
-          }
-          neg_m = -m;
+          raise();
         }
         // P = 2^(s c - m) as packed bf16.  (Probabilities meet the values as bf16, the type of the tensor cores' other operand; their sum stays in
         // fp32.)
-        float sum0 = 0.f, sum1 = 0.f;
         if (active) {
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
@@ -781,32 +866,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         // the product before has read P, and O is complete
         if (my_turn > 0 && !(ok = wait(&o_done[t], (uint32_t)((my_turn - 1) & 1), 332))) break;
-        if (active && __any_sync(0xffffffffu, rescale)) {
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {                     // narrow pieces: the scores stay in registers meanwhile
-            uint32_t o[16];
-            tmem_ld_32x16(o_addr + c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st_32x16(o_addr + c, o);
-          }
-          l *= alpha;
-        }
-        if (kv0 + 128 > w.s.ctx && (!pair || t == 0 || i >= n[0])) {
-          // Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them (by
-          // the chain whose product comes first).
-          // (what stood in the slot before has been used, so that the parity is that of this page)
-          if (i == 0 && pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
-          const int slot = RING + (done + g) % RING;
-          if (!(ok = wait(&full[slot], (uint32_t)(((done + g) / RING) & 1), 330))) break;
-          if (kv0 + row >= w.s.ctx) {
-#pragma unroll
-            for (int d = 0; d < D / 8; ++d) *reinterpret_cast<uint4*>(ring + slot * TILE + (d / 8) * SLAB + row * 128 + (d % 8) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_async_proxy();
-        }
+        if (active && __any_sync(0xffffffffu, rescale)) rescale_sums();
+        if (unclean && !(ok = clear_values())) break;
         if (active) {
           tmem_st_32x32(p_addr, r);
           tmem_st_32x32(p_addr + 32, r + 32);
@@ -814,7 +875,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (!ok) break;
         l += sum0 + sum1;
       }
-      if (ok && mine > 0) hand_over();
+      if (!FEW && ok && mine > 0) hand_over();
       if (!ok) break;
       done += w.nb;
       turns[0] += n[0];
