@@ -773,16 +773,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           if (!(ok = wait(&s_full[t], (uint32_t)(my_turn & 1), 329))) break;
           tc_fence_after();
           if (active) {
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-              uint32_t r[32];
-              tmem_ld_32x32(s_addr + c, r);
-              tmem_wait_ld();
-              if (masked) {
+            // columns that no row of the tile, and that not every row sees, in whole 32s
+            const int columns = min(128, (hidden - kv0 + w.s.n - 1) / 32 * 32 + 32), clear = hidden - kv0 - 31;
+            auto mask = [&](int c, uint32_t* r) {
+              if (c <= clear) return;
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (e > lim - c) r[e] = __float_as_uint(-1e30f);
-              }
+              for (int e = 0; e < 32; ++e)
+                if (e > lim - c) r[e] = __float_as_uint(-1e30f);
+            };
+            auto largest = [&](int c, uint32_t* r) {
+              mask(c, r);
 #pragma unroll
               for (int e = 0; e < 32; e += 8) {
                 mx0 = pa_max3(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
@@ -790,19 +790,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 mx2 = pa_max3(mx2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
                 mx3 = pa_max3(mx3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
               }
-            }
-            raise();
-            if (__any_sync(0xffffffffu, rescale)) rescale_sums();      // (the product before is complete, or there were no scores)
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-              uint32_t r[32];
-              tmem_ld_32x32(s_addr + c, r);
-              tmem_wait_ld();
-              if (masked) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (e > lim - c) r[e] = __float_as_uint(-1e30f);
-              }
+            };
+            auto exponentials = [&](int c, uint32_t* r) {
+              mask(c, r);
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 float x0, x1;
@@ -812,6 +802,26 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 r[e] = pack_bf16(e0, e1);
               }
               tmem_st_32x16(p_addr + c / 2, r);
+            };
+            auto columns_by = [&](auto&& work) {
+#pragma unroll 1
+              for (int c = 0; c < columns; c += 32) {
+                uint32_t r[32];
+                tmem_ld_32x32(s_addr + c, r);
+                tmem_wait_ld();
+                work(c, r);
+              }
+            };
+            columns_by(largest);
+            raise();
+            if (__any_sync(0xffffffffu, rescale)) rescale_sums();      // (the product before is complete, or there were no scores)
+            columns_by(exponentials);
+#pragma unroll 1
+            for (int c = columns; c < 128; c += 32) {
+              uint32_t none[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) none[e] = 0;
+              tmem_st_32x16(p_addr + c / 2, none);
             }
           }
           if (unclean && !(ok = clear_values())) break;
