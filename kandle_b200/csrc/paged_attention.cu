@@ -18,11 +18,14 @@
 // (with P over S it waited for P V, and a chain's step was the sum of both: 4331 cycles for two tiles and a page, of which the exponential unit
 // needs 2048 and the tensor pipe 2048).  Tensor memory holds one S for both chains, which they use in turn, two P and two O.  Two threads a
 // row (and 16 warps) were slower: they have to exchange the maximum.  With up to 32 rows (FEW) one warp has a tile, and its instructions have to come
-// for it alone: short loops over 32 scores at a time, P over S.
+// for it alone: short loops over 32 scores at a time, P over S; with up to 16 rows a thread has a quarter of the scores of one or two rows, so that lanes
+// without a row have no exponentials (32 single tokens: 84.1 us with a row's 128 scores in straight code, 80.3 in loops, 75.0 so).
 //
-// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 80 us, 4.7 TB/s, of which some 20 are the launch, the division,
+// Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 75 us, 5.1 TB/s, of which some 15 are the launch, the division,
 // the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 44 us; 4 x 2048 tokens on 6144 (32 on 8) 1000 us,
 // 960 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
@@ -92,6 +95,22 @@ __device__ __forceinline__ void pa_fma2(float& x0, float& x1, float a0, float a1
 __device__ __forceinline__ void pa_add2(float& s0, float& s1, float a0, float a1) {
   asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
+}
+
+// 16 lanes x 32 columns: thread i receives, of lanes i / 4 and i / 4 + 8, columns 8 g + 2 (i % 4) and the next, as r[4 g .. 4 g + 1] and r[4 g + 2 .. 4 g + 3].
+__device__ __forceinline__ void pa_ld_16x32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 lanes x 16 columns: thread i has column 4 g + i % 4 of lanes i / 4 and i / 4 + 8 as r[2 g] and r[2 g + 1].
+__device__ __forceinline__ void pa_st_16x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // ----------------------------------------------------------------------------- the division of the work
@@ -696,7 +715,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     if constexpr (!FEW) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFTMAX_REGS));
     const int t = warp >> 2, q = warp & 3, row = q * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16), s_addr = lane_addr + (uint32_t)t * S_STEP, p_addr = lane_addr + P_COL + (uint32_t)t * P_STEP, o_addr = lane_addr + O_COL + (uint32_t)(t * D);
-    const int row_token = row / group;
+    const int row_token = row / group, slim_token1 = FEW ? (lane >> 2) / group : 0, slim_token2 = FEW ? ((lane >> 2) + 8) / group : 0;
     int done = 0, pieces = 0, turns[2] = {0, 0}, y_turn = 0;
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -714,6 +733,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       const int mine = t ? n[1] : n[0];
       int my_turn = t ? turns[1] : turns[0];
       float m = -1e30f, l = 0.f;
+      // FEW, up to 16 rows: a thread has a quarter of the columns of rows lane / 4 and lane / 4 + 8 (whose statistics are m2 and l2)
+      const bool slim = FEW && rows <= 16;
+      const int last1 = (lane >> 2) < rows ? hidden + slim_token1 : -1, last2 = (lane >> 2) + 8 < rows ? hidden + slim_token2 : -1;
+      float m2 = -1e30f, l2 = 0.f;
       // P, and values that were cleared, are there for the product
       auto hand_over = [&] {
         if (active) tmem_wait_st();
@@ -750,7 +773,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
             tmem_st_32x16(o_addr + c, o);
           }
-          l *= alpha;
         };
         // Behind the last key a page may hold anything, and 0 x NaN is none: those values become zeros before a product reads them (by
         // the chain whose product comes first).
@@ -812,10 +834,86 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 work(c, r);
               }
             };
-            columns_by(largest);
-            raise();
-            if (__any_sync(0xffffffffu, rescale)) rescale_sums();      // (the product before is complete, or there were no scores)
-            columns_by(exponentials);
+            // As above for up to 16 rows, TWO: more than 8.
+            auto slim_tile = [&](auto two) {
+              constexpr bool TWO = decltype(two)::value;
+              const int lim1 = last1 - kv0 - 2 * (lane & 3), lim2 = last2 - kv0 - 2 * (lane & 3);
+              float x[2][2] = {{-1e30f, -1e30f}, {-1e30f, -1e30f}}, sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}}, alpha2 = 1.f;
+              auto slim_mask = [&](int c, uint32_t* r) {
+                if (c <= clear) return;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  if (e % 4 < 2 && 8 * (e / 4) + e % 2 > lim1 - c) r[e] = __float_as_uint(-1e30f);
+                  if (TWO && e % 4 >= 2 && 8 * (e / 4) + e % 2 > lim2 - c) r[e] = __float_as_uint(-1e30f);
+                }
+              };
+#pragma unroll 1
+              for (int c = 0; c < columns; c += 32) {
+                uint32_t r[16];
+                pa_ld_16x32(s_addr + c, r);
+                tmem_wait_ld();
+                slim_mask(c, r);
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                  x[0][e / 4 % 2] = pa_max3(x[0][e / 4 % 2], __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+                  if (TWO) x[1][e / 4 % 2] = pa_max3(x[1][e / 4 % 2], __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+                }
+              }
+              auto slim_raise = [&](float (&y)[2], bool some, float& m, float& alpha) {
+                float now = fmaxf(y[0], y[1]);
+                now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 1));
+                now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2)) * p.scale_log2;
+                if (i == 0 || !some) {
+                  m = now;
+                } else if (now - m > 8.0f) {
+                  alpha = pa_exp2(m - now);
+                  m = now;
+                  rescale = true;
+                }
+              };
+              slim_raise(x[0], last1 >= 0, m, alpha);
+              if (TWO) slim_raise(x[1], last2 >= 0, m2, alpha2);
+              if (__any_sync(0xffffffffu, rescale)) {
+                l *= alpha;
+                l2 *= alpha2;
+                const float a1 = __shfl_sync(0xffffffffu, alpha, (lane & 7) * 4), a2 = __shfl_sync(0xffffffffu, alpha2, (lane & 7) * 4);
+                alpha = lane < 8 ? a1 : a2;                           // of row `lane`
+                rescale_sums();
+              }
+#pragma unroll 1
+              for (int c = 0; c < columns; c += 32) {
+                uint32_t r[16], y[8];
+                pa_ld_16x32(s_addr + c, r);
+                tmem_wait_ld();
+                slim_mask(c, r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  if (e % 2 == 1 && !TWO) { y[e] = 0; continue; }
+                  float x0, x1;
+                  pa_fma2(x0, x1, __uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), p.scale_log2, e % 2 ? -m2 : -m);
+                  const float e0 = pa_exp2(x0), e1 = pa_exp2(x1);
+                  pa_add2(sum[e % 2][0], sum[e % 2][1], e0, e1);
+                  y[e] = pack_bf16(e0, e1);
+                }
+                pa_st_16x16(p_addr + c / 2, y);
+              }
+              l += sum[0][0] + sum[0][1];
+              l2 += sum[1][0] + sum[1][1];
+            };
+            if (rows <= 8) {
+              slim_tile(std::false_type{});
+            } else if (rows <= 16) {
+              slim_tile(std::true_type{});
+            } else {
+              columns_by(largest);
+              raise();
+              if (__any_sync(0xffffffffu, rescale)) {                   // (the product before is complete, or there were no scores)
+                rescale_sums();
+                l *= alpha;
+              }
+              columns_by(exponentials);
+              l += sum0 + sum1;
+            }
 #pragma unroll 1
             for (int c = columns; c < 128; c += 32) {
               uint32_t none[16];
@@ -826,7 +924,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           if (unclean && !(ok = clear_values())) break;
           hand_over();
-          l += sum0 + sum1;
           continue;
         }
         uint32_t r[128];
@@ -876,7 +973,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         // the product before has read P, and O is complete
         if (my_turn > 0 && !(ok = wait(&o_done[t], (uint32_t)((my_turn - 1) & 1), 332))) break;
-        if (active && __any_sync(0xffffffffu, rescale)) rescale_sums();
+        if (active && __any_sync(0xffffffffu, rescale)) {
+          rescale_sums();
+          l *= alpha;
+        }
         if (unclean && !(ok = clear_values())) break;
         if (active) {
           tmem_st_32x32(p_addr, r);
@@ -892,7 +992,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       turns[1] += n[1];
       // a row that sees none of the chain's keys has summed masked ones
       const int first_key = (w.j0 + (pair ? 0 : t)) * 128;
-      if (mine == 0 || last < first_key) { m = -1e30f; l = 0.f; }
+      if (mine == 0 || (slim ? last1 : last) < first_key) { m = -1e30f; l = 0.f; }
       float2* now = ml + (pieces & 1) * 2 * PA_ROWS;
       if constexpr (FEW) {
         const bool some = w.nb > 0;
@@ -901,7 +1001,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (q == 0) {
           // (the outputs of the piece before have been read: nobody is two pieces ahead)
           if (pieces > 0 && !(ok = wait(o_free, (uint32_t)((pieces - 1) & 1), 333))) break;
-          now[t * PA_ROWS + row] = make_float2(m, l);
+          if (slim) {
+            if (mine == 0 || last2 < first_key) { m2 = -1e30f; l2 = 0.f; }
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l2 += __shfl_xor_sync(0xffffffffu, l2, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            l2 += __shfl_xor_sync(0xffffffffu, l2, 2);
+            if (lane % 4 == 0) {
+              now[t * PA_ROWS + lane / 4] = make_float2(m, l);
+              now[t * PA_ROWS + lane / 4 + 8] = make_float2(m2, l2);
+            }
+          } else {
+            now[t * PA_ROWS + row] = make_float2(m, l);
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(few_done);
         }
