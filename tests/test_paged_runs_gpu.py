@@ -209,6 +209,35 @@ def test_vocabularies_beyond_two_to_the_30_are_refused(backend):
     logits.dispose()
 
 
+@pytest.mark.parametrize("pdl", [0, 1])
+def test_a_captured_call_of_two_kernels(backend, pdl):
+    """A prompt that is cut into parts of two tiles beside a few tokens; replayed with other lengths and after a call that leaves other parts."""
+    a = attention_case([300, 5], [1500, 130], 4, 2, 64, seed=1, table_width=14, spare_pages=9)
+    b = attention_case([290, 15], [300, 1700], 4, 2, 64, seed=2, table_width=14, spare_pages=6)
+    assert a["k"].shape == b["k"].shape and a["q"].shape == b["q"].shape
+    d = {n: put(a[n]) for n in ("q", "k", "v", "table", "keys", "start")}
+    out = core.empty(tuple(a["q"].shape), "bfloat16")
+    call = lambda: paged.attention(d["q"], d["k"], d["v"], d["table"], d["keys"], q_start=d["start"], scale=a["scale"], out=out)  # noqa: E731
+    call()
+    check(a, out.dataAsync())
+    lib.call("kd_graph_begin")
+    lib.call("kd_set_pdl", pdl)
+    try:
+        call()
+    finally:
+        lib.call("kd_set_pdl", 0)
+    g = ctypes.c_uint64(0)
+    lib.call("kd_graph_end", ctypes.byref(g))
+    other = attention_case([700, 1, 90], [900, 2000, 400], 8, 2, 128, seed=3)
+    for c in (b, a, b):
+        for n in d:
+            core.copy_(d[n], put(c[n]))
+        check(other, run(other))
+        lib.call("kd_graph_launch", g)
+        check(c, out.dataAsync())
+    lib.call("kd_graph_destroy", g)
+
+
 def test_command_line_searches_with_beams(backend, tmp_path):
     w = {k: lib.round_to_bf16(v) for k, v in synth.qwen3_weights(std=0.05, head_dim=64, **DIMS).items()}
     (tmp_path / "config.json").write_text(json.dumps({"architectures": ["Qwen3ForCausalLM"], "vocab_size": 1024, "hidden_size": 256, "intermediate_size": 512, "num_hidden_layers": 3,
