@@ -38,7 +38,7 @@ import numpy as np
 from . import core, lib, paged, parallel
 from .core import Tensor
 from .model_utils.qwen3 import Qwen3Config
-from .model_utils.sampling import beam_select
+from .model_utils.sampling import BeamHypotheses, beam_select
 
 
 def _r(t):
@@ -714,7 +714,7 @@ class Qwen3Engine(DecoderEngine):
         """Beam search behind prompts ids [B,S] (paged cache, B * beams <= max_batch): up to `steps` tokens.  Returns, per prompt, up to `beams`
         hypotheses (tokens, score), best first; score is the sum of the tokens' log-probabilities divided by their number to the power
         length_penalty.  One that ends with `eos` leaves its beam to others; a prompt is done when `beams` have ended and the best running one
-        scores no higher than the worst of them.  Beams share the pages that they have in common.  The cache is free afterwards."""
+        scores no higher than the worst of them, and keeps its hypotheses of that step while other prompts go on.  Beams share the pages that they have in common.  The cache is free afterwards."""
         if not self.paged:
             raise ValueError("beams need a paged cache (paged=True)")
         if self.tp > 1:
@@ -758,22 +758,14 @@ class Qwen3Engine(DecoderEngine):
         self._place(d)
         self._beam_step(b)
         d["beams"], d["use_graph"] = b, use_graph
-        running, ended = [[[]] * K for _ in range(B)], [[] for _ in range(B)]
-
-        def worth(score: float, n: int) -> float:
-            return float(score) / n ** power
-
+        prompts = [BeamHypotheses(K, eos, power) for _ in range(B)]
         for step in range(1, steps + 1):
-            parents, tokens, scores, ends = (b[n].dataAsync() for n in ("parents", "tokens", "scores", "ended"))
-            for i in range(B):
-                for j in np.flatnonzero(np.isfinite(ends[i])):
-                    ended[i].append((running[i][j] + [eos], worth(ends[i, j], step)))
-                ended[i] = sorted(ended[i], key=lambda h: -h[1])[:K]
-                running[i] = [running[i][p] + [int(t)] for p, t in zip(parents[i], tokens[i])]
-            done = [len(e) == K and e[-1][1] >= worth(s[0], step) for e, s in zip(ended, scores)]
-            if step == steps or all(done):
+            outputs = [b[n].dataAsync() for n in ("parents", "tokens", "scores", "ended")]
+            for i, prompt in enumerate(prompts):
+                prompt.step(*(o[i] for o in outputs))
+            if step == steps or all(prompt.done for prompt in prompts):
                 break
             if self.pos % paged.PAGE == 0:
                 self._fresh_pages(b, book, table, self.pos // paged.PAGE)
             self.decode_step()
-        return [sorted(e + [(r, worth(s, len(r))) for r, s in zip(rs, ss) if np.isfinite(s)], key=lambda h: -h[1])[:K] for e, rs, ss in zip(ended, running, scores)]
+        return [prompt.best() for prompt in prompts]

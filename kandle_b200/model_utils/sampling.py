@@ -78,3 +78,33 @@ def beam_select(logits: Tensor, scores: Tensor, eos: int = -1, out=None):
     new, parents, tokens, ended = out
     lib.call("kd_beam_select", _r(logits), _r(scores), int(eos), _r(new), _r(parents), _r(tokens), _r(ended))
     return out
+
+
+class BeamHypotheses:
+    """What a beam search keeps of ONE prompt on the host: the running beams' tokens and the best `beams` hypotheses that ended.  A hypothesis of n
+    tokens with log-probability s is worth s / n ** power.  The prompt is done when `beams` have ended and the best running one is worth no more
+    than the worst of them; what comes later, because other prompts of the batch go on, changes nothing any more."""
+
+    def __init__(self, beams: int, eos: int, power: float):
+        self.beams, self.eos, self.power = beams, eos, power
+        self.running, self.scores, self.ended, self.done = [[] for _ in range(beams)], [], [], False
+
+    def _worth(self, score: float, n: int) -> float:
+        return float(score) / n ** self.power
+
+    def step(self, parents, tokens, scores, ends) -> None:
+        """A step's outputs of beam_select for this prompt, each [beams]."""
+        if self.done:
+            return
+        n = len(self.running[0]) + 1
+        for j in np.flatnonzero(np.isfinite(ends)):
+            self.ended.append((self.running[j] + [self.eos], self._worth(ends[j], n)))
+        self.ended = sorted(self.ended, key=lambda h: -h[1])[:self.beams]
+        self.running = [self.running[p] + [int(t)] for p, t in zip(parents, tokens)]
+        self.scores = [float(s) for s in scores]
+        self.done = len(self.ended) == self.beams and self.ended[-1][1] >= self._worth(scores[0], n)
+
+    def best(self) -> list:
+        """Up to `beams` (tokens, worth), best first."""
+        going = [] if self.done else [(r, self._worth(s, len(r))) for r, s in zip(self.running, self.scores) if np.isfinite(s)]
+        return sorted(self.ended + going, key=lambda h: -h[1])[:self.beams]

@@ -104,3 +104,30 @@ def fork_answer(pools, parents, table, spare, length):
             seen.add(p)
             table[r, whole] = page
     return table, spare
+
+
+def beam_rule(outputs, beams, eos, steps, power):
+    """The rule of Qwen3Engine.generate_beams for one prompt, over the outputs of its steps (scores, parents, tokens, ended), each [beams].
+    Returns the hypotheses (tokens, worth), best first, and the step in which the prompt was done (None: it was not)."""
+    tokens, ended = [[]] * beams, []
+    for step, (s, parents, new, ends) in enumerate(outputs, 1):
+        ended += [(tokens[j] + [eos], ends[j] / step ** power) for j in range(beams) if np.isfinite(ends[j])]
+        ended = sorted(ended, key=lambda h: -h[1])[:beams]
+        tokens = [tokens[p] + [int(t)] for p, t in zip(parents, new)]
+        if len(ended) == beams and s[0] / step ** power <= ended[-1][1]:
+            return ended, step
+        if step == steps:
+            break
+    return sorted(ended + [(t, x / steps ** power) for t, x in zip(tokens, s) if np.isfinite(x)], key=lambda h: -h[1])[:beams], None
+
+
+def beam_search(logits_of, beams, eos, steps, power):
+    """beam_rule with float64's choice.  logits_of: the beams' tokens -> logits [beams, V]."""
+    def outputs():
+        tokens, scores = [[]] * beams, np.full((1, beams), -np.inf)
+        scores[0, 0] = 0
+        while True:
+            s, parents, new, ends = beam_answer(logits_of(tokens)[None], scores, eos)
+            yield s[0], parents[0], new[0], ends[0]
+            tokens, scores = [tokens[p] + [int(t)] for p, t in zip(parents[0], new[0])], s
+    return beam_rule(outputs(), beams, eos, steps, power)
