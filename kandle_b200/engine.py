@@ -363,10 +363,12 @@ class Qwen3Engine(DecoderEngine):
         if portion is not None and portion < 1:
             raise ValueError(f"portions of {portion} tokens")
         if portion is not None and portion < ids.shape[1]:
-            if ids.shape[1] > self.max_seq_len:
-                raise ValueError(f"prefill of {ids.shape[0]}x{ids.shape[1]} exceeds the engine's {self.B}x{self.max_seq_len}")
+            B, S = ids.shape
+            if S > self.max_seq_len:
+                raise ValueError(f"prefill of {B}x{S} exceeds the engine's {self.B}x{self.max_seq_len}")
             host = ids.dataAsync() if isinstance(ids, Tensor) else np.asarray(ids)
-            parts = [(self.extend if a else self.prefill)(np.ascontiguousarray(host[:, a:a + portion]), all_logits) for a in range(0, host.shape[1], portion)]
+            # only the last portion has a next token (and draws its random numbers)
+            parts = [self._run_prompt(host[:, a:a + portion], a, all_logits, a + portion >= S) for a in range(0, S, portion)]
             return (parts[-1][0], core.cat([p[1] for p in parts], 1)) if all_logits else parts[-1]
         return self._run_prompt(ids, 0, all_logits)
 
@@ -380,7 +382,7 @@ class Qwen3Engine(DecoderEngine):
             raise ValueError(f"Cache overflow: trying to write to position {self.pos}-{self.pos + ids.shape[1]}, but maxSeqLen is {self.max_seq_len}")
         return self._run_prompt(ids, self.pos, all_logits)
 
-    def _run_prompt(self, ids, start: int, all_logits: bool):
+    def _run_prompt(self, ids, start: int, all_logits: bool, last: bool = True):
         if isinstance(ids, Tensor):
             B, S = ids.shape
             ids_t = ids.view(B * S)
@@ -399,7 +401,7 @@ class Qwen3Engine(DecoderEngine):
         # 2560 wide, 9 layers: 1024 2.62, 2.49; 3 x 701 4.52, 4.46)
         lib.call("kd_set_pdl", 3 if self.use_pdl and self.tp == 1 and B * S <= 16384 else 0)
         try:
-            full = self._prefill_kernels(w, ids_t, B, S, start, all_logits)
+            full = self._prefill_kernels(w, ids_t, B, S, start, all_logits, last)
         finally:
             lib.call("kd_set_pdl", 0)
         self.pos = start + S
@@ -425,7 +427,7 @@ class Qwen3Engine(DecoderEngine):
         kc.dispose()
         vc.dispose()
 
-    def _prefill_kernels(self, w: dict, ids_t: Tensor, B: int, S: int, start: int, all_logits: bool):
+    def _prefill_kernels(self, w: dict, ids_t: Tensor, B: int, S: int, start: int, all_logits: bool, next_tokens: bool):
         c = self.cfg
         T = B * S
         core._kernel("index_select")(self.embed._handle, ids_t._handle, {"dim": 0}, w["emb"]._handle)
@@ -487,17 +489,19 @@ class Qwen3Engine(DecoderEngine):
                 self._norm(w["part"], nxt, w["x"], resid=h1, sum_out=h)
             kc.dispose()
             vc.dispose()
-        # tied lm_head on the last position of every sequence (select commutes with the row-wise matmul)
-        h3 = h.view(B, S, self.H)
-        last = h3.select(1, S - 1)
-        core.copy_(w["last"], last)
-        self._norm(w["last"], self.final_norm, w["xl"])
-        lib.call("kd_linear_bf16_skinny", _r(w["xl"]), _r(self.embed), 0, _r(w["logits"]))
-        lg = w["logits"].view(B, self.V)
-        if self.sampler is not None:
-            self._fresh_uniforms(w["uniforms"])
-        self._next_tokens(lg, w["uniforms"], w["tok"])
-        lg.dispose()
+        if next_tokens:
+            # tied lm_head on the last position of every sequence (select commutes with the row-wise matmul)
+            h3 = h.view(B, S, self.H)
+            last = h3.select(1, S - 1)
+            core.copy_(w["last"], last)
+            self._norm(w["last"], self.final_norm, w["xl"])
+            lib.call("kd_linear_bf16_skinny", _r(w["xl"]), _r(self.embed), 0, _r(w["logits"]))
+            lg = w["logits"].view(B, self.V)
+            if self.sampler is not None:
+                self._fresh_uniforms(w["uniforms"])
+            self._next_tokens(lg, w["uniforms"], w["tok"])
+            for t in (h3, last, lg):
+                t.dispose()
         full = None
         if all_logits:
             xa = core.empty((T, self.H), "bfloat16")
@@ -505,7 +509,7 @@ class Qwen3Engine(DecoderEngine):
             full = core.empty((B, S, self.V), "float32")
             self._linear(xa, self.embed, full)
             xa.dispose()
-        for t in (q_bhsd, o_bhsd, attn2d, h3, last, *([ctx] if ctx is not None else [])):
+        for t in (q_bhsd, o_bhsd, attn2d, *([ctx] if ctx is not None else [])):
             t.dispose()
         if table is not None:
             table.dispose()
