@@ -697,28 +697,36 @@ class Qwen3Engine(DecoderEngine):
     def _beam_state(self, d: dict, B: int, K: int, eos: int) -> dict:
         R = B * K
         return {"key": (B, K, eos), "scores": core.zeros((B, K), "float32"), "parents": core.zeros((B, K), "int32"), "ended": core.zeros((B, K), "float32"),
-                "spare": core.zeros((R,), "int32"), "logits": d["logits"].view(B, K, self.V), "tokens": d["ids"].view(B, K),
-                "table": self.block_table.slice([slice(0, R), slice(None)]), "length": d["pos"], "pools": paged.Pools([*self.k_cache, *self.v_cache])}
+                "spare": core.zeros((R,), "int32"), "logits": d["logits"].view(B, K, self.V), "tokens": d["ids"].view(B, K), "length": d["pos"]}
+
+    def _beam_table(self, b: dict) -> Tensor:
+        return self.block_table.slice([slice(0, b["spare"].shape[0]), slice(None)])
 
     def _beam_step(self, b: dict) -> None:
-        """The beams' next tokens, and the cache that stands behind each."""
+        """The beams' next tokens, and the cache that stands behind each.  The pools' descriptors are laid out for every call, as the layers' are:
+        the engine may have been given other caches since the last one."""
         beam_select(b["logits"], b["scores"], b["key"][2], out=(b["scores"], b["parents"], b["tokens"], b["ended"]))
-        paged.fork_pages(b["pools"], b["parents"], b["table"], b["spare"], b["length"])
+        table = self._beam_table(b)
+        paged.fork_pages([*self.k_cache, *self.v_cache], b["parents"], table, b["spare"], b["length"])
+        table.dispose()
 
     def _fresh_pages(self, b: dict, book: paged.PagePool, table: np.ndarray, column: int) -> None:
         """Every beam gets a page of its own for the positions from 128 * column on.  What the beams no longer name is free."""
-        R = len(table)
+        rows = self._beam_table(b)
         spare = b["spare"].dataAsync()
-        table[:, :column] = b["table"].dataAsync()[:, :column]
+        table[:, :column] = rows.dataAsync()[:, :column]
         book.keep(np.concatenate([table[:, :column].reshape(-1), spare]))
-        table[:, column] = book.take(R)
-        core._backend().upload(b["table"]._handle, table)
+        table[:, column] = book.take(len(table))
+        core._backend().upload(rows._handle, table)
+        rows.dispose()
 
     def generate_beams(self, ids, beams: int, steps: int, eos: int = -1, length_penalty: float = 1.0, use_graph: bool = True) -> list:
         """Beam search behind prompts ids [B,S] (paged cache, B * beams <= max_batch): up to `steps` tokens.  Returns, per prompt, up to `beams`
         hypotheses (tokens, score), best first; score is the sum of the tokens' log-probabilities divided by their number to the power
         length_penalty.  One that ends with `eos` leaves its beam to others; a prompt is done when `beams` have ended and the best running one
-        scores no higher than the worst of them, and keeps its hypotheses of that step while other prompts go on.  Beams share the pages that they have in common.  The cache is free afterwards."""
+        scores no higher than the worst of them, and keeps its hypotheses of that step while other prompts go on.  Beams share the pages that they
+        have in common.  The cache is free afterwards.  (With use_graph the step is captured as generate's is: dispose() after putting other
+        weights or caches into the engine.)"""
         if not self.paged:
             raise ValueError("beams need a paged cache (paged=True)")
         if self.tp > 1:
@@ -752,7 +760,9 @@ class Qwen3Engine(DecoderEngine):
         if whole < held:
             table[np.arange(R) % K != 0, whole] = book.take(R - B)
         core._backend().upload(b["spare"]._handle, book.take(R))
-        core._backend().upload(b["table"]._handle, table)
+        rows = self._beam_table(b)
+        core._backend().upload(rows._handle, table)
+        rows.dispose()
         logits = b["logits"].select(1, 0)
         core.copy_(logits, self._prefill_bufs[(B, S)]["logits"].view(B, self.V))
         logits.dispose()

@@ -1,0 +1,38 @@
+"""Qwen3Engine.generate_beams: what an engine keeps from one search to the next."""
+import numpy as np
+import pytest
+
+from kandle_b200 import core, lib, synth
+from kandle_b200.core import Tensor
+from kandle_b200.engine import Qwen3Engine
+from kandle_b200.model_utils.qwen3 import Qwen3Config
+
+pytestmark = pytest.mark.gpu
+
+K, STEPS = 4, 12
+
+
+def engine(batch=8, room=256, **more):
+    dims = dict(vocab=512, hidden=256, inter=512, layers=2, heads=4, kv_heads=2)
+    w = {k: lib.round_to_bf16(v) for k, v in synth.qwen3_weights(std=0.05, head_dim=128, **dims).items()}
+    cfg = Qwen3Config(vocabSize=512, hiddenSize=256, intermediateSize=512, numHiddenLayers=2, numAttentionHeads=4, numKeyValueHeads=2, headDim=128, dtype="bfloat16")
+    return Qwen3Engine(cfg, w, batch, room, paged=True, spare_pages=2 * batch, **more)
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_beams_go_through_the_caches_and_the_table_that_the_engine_has_now(backend, use_graph):
+    """Steps without a graph read the engine's tensors at every call; captured ones after dispose()."""
+    eng = engine()
+    ids = synth.token_ids("beams.swap", (2, 120), 512)
+    want = eng.generate_beams(ids, K, STEPS, use_graph=use_graph)
+    old = [*eng.k_cache, *eng.v_cache]
+    before, table = [t.dataAsync() for t in old], eng.block_table
+    eng.k_cache, eng.v_cache = ([core.zeros(t.shape, "bfloat16") for t in c] for c in (eng.k_cache, eng.v_cache))
+    eng.block_table = Tensor(table.dataAsync())
+    if use_graph:
+        eng.dispose()
+    assert eng.generate_beams(ids, K, STEPS, use_graph=use_graph) == want
+    for a, t in zip(before, old):
+        assert np.array_equal(a, t.dataAsync()), "nothing is written where the engine was before"
+    assert any(t.dataAsync().any() for t in eng.k_cache)
+    eng.dispose()
