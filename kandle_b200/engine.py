@@ -532,7 +532,7 @@ class Qwen3Engine(DecoderEngine):
             return s.value
         p2p = self.tp > 1 and self.use_p2p and parallel.peer_buffers_ready()
         d = {
-            "B": B, "graph": {}, "beams": None, "chain": self.use_chain,
+            "B": B, "graph": {}, "beams": None, "beam_state": None, "chain": self.use_chain,
             # (tensor parallel: fp32 partial sums of all sequences must fit one 2 MiB exchange slot)
             "fused": self.use_fused_layer and (self.tp == 1 or (p2p and B * self.H * 4 <= (2 << 20))),
             "p2p": p2p,
@@ -695,9 +695,15 @@ class Qwen3Engine(DecoderEngine):
 
     # ------------------------------------------------------------------ beams
     def _beam_state(self, d: dict, B: int, K: int, eos: int) -> dict:
+        """The buffers of a search, kept (with the captured steps that write them) for the next one of the same kind only."""
         R = B * K
-        return {"key": (B, K, eos), "scores": core.zeros((B, K), "float32"), "parents": core.zeros((B, K), "int32"), "ended": core.zeros((B, K), "float32"),
+        if d["beam_state"] is not None and d["beam_state"]["key"] == (B, K, eos):
+            return d["beam_state"]
+        for form in [f for f in d["graph"] if isinstance(f, tuple)]:
+            lib.call("kd_graph_destroy", ctypes.c_uint64(d["graph"].pop(form)))
+        d["beam_state"] = {"key": (B, K, eos), "scores": core.zeros((B, K), "float32"), "parents": core.zeros((B, K), "int32"), "ended": core.zeros((B, K), "float32"),
                 "spare": core.zeros((R,), "int32"), "logits": d["logits"].view(B, K, self.V), "tokens": d["ids"].view(B, K), "length": d["pos"]}
+        return d["beam_state"]
 
     def _beam_table(self, b: dict) -> Tensor:
         return self.block_table.slice([slice(0, b["spare"].shape[0]), slice(None)])
@@ -750,8 +756,7 @@ class Qwen3Engine(DecoderEngine):
     def _generate_beams(self, ids, B: int, S: int, K: int, R: int, steps: int, eos: int, power: float, use_graph: bool) -> list:
         self.prefill(ids)
         d = self._decode_state(R)
-        states = d.setdefault("beam_states", {})
-        b = states.get((B, K, eos)) or states.setdefault((B, K, eos), self._beam_state(d, B, K, eos))
+        b = self._beam_state(d, B, K, eos)
         # the prompt's pages stand in the first beam's row; the others take them over as children of it
         book, held, whole = paged.PagePool(self.k_cache[0].shape[0]), -(-S // paged.PAGE), S // paged.PAGE
         book.keep(self.page_table[:B, :held])

@@ -36,3 +36,24 @@ def test_beams_go_through_the_caches_and_the_table_that_the_engine_has_now(backe
         assert np.array_equal(a, t.dataAsync()), "nothing is written where the engine was before"
     assert any(t.dataAsync().any() for t in eng.k_cache)
     eng.dispose()
+
+
+def test_searches_of_many_kinds_leave_nothing_behind(backend, collected):
+    """Other end tokens and other numbers of beams: the captured steps and buffers of one kind are kept, not of all."""
+    eng = engine()
+    ids = synth.token_ids("beams.kinds", (2, 100), 512)
+    want = {}
+    kinds = [(2, 4, -1), (2, 4, 3), (2, 4, 500), (1, 8, -1), (2, 4, 77), (1, 8, 9)]
+    for turn in range(2):
+        for n, k, eos in kinds:
+            got = eng.generate_beams(ids[:n], k, STEPS, eos)
+            assert want.setdefault((n, k, eos), got) == got
+            assert len(eng._decode["graph"]) <= 2
+        used = backend.memory_stats()
+        if turn == 0:
+            first = used
+    assert used == first
+    want = eng.generate(np.repeat(ids, 4, 0), 5)
+    eng.generate_beams(ids, 4, STEPS, 5)
+    assert np.array_equal(eng.generate(np.repeat(ids, 4, 0), 5), want), "the captured step of the plain generation is another one"
+    eng.dispose()
