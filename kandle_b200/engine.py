@@ -244,7 +244,6 @@ class Qwen3Engine(DecoderEngine):
             if page_table.shape != (self.B, per_seq) or page_table.min() < 0 or len(np.unique(page_table)) != n_pages:
                 raise ValueError(f"page_table must hold {n_pages} distinct page indices in a [{self.B},{per_seq}] array")
             n_pool = int(page_table.max()) + 1 + int(spare_pages)
-            self.page_table = page_table
             self.block_table = Tensor(page_table)
             # pools [pages,Hkv,128,D] per layer, zero-initialised like the contiguous cache
             self.k_cache = [core.zeros((n_pool, self.Hkv, 128, self.D), "bfloat16") for _ in range(self.L)]
@@ -743,25 +742,26 @@ class Qwen3Engine(DecoderEngine):
             raise ValueError(f"{B} prompts of {S} tokens with {K} beams and {steps} steps: 1 to 32 beams, at most {self.B} in all, and one step at least")
         if S + steps > self.max_seq_len:
             raise ValueError(f"Cache overflow: {S} + {steps} positions, but maxSeqLen is {self.max_seq_len}")
+        own = self.block_table.dataAsync()
         sampler, self.sampler = self.sampler, None
         try:
-            return self._generate_beams(ids, B, S, K, R, steps, int(eos), float(length_penalty), use_graph)
+            return self._generate_beams(ids, own, B, S, K, R, steps, int(eos), float(length_penalty), use_graph)
         finally:
             self.sampler = sampler
-            core._backend().upload(self.block_table._handle, self.page_table)
+            core._backend().upload(self.block_table._handle, own)
             if self._decode is not None:
                 self._decode["beams"] = None
             self.pos = self.cur_B = 0
 
-    def _generate_beams(self, ids, B: int, S: int, K: int, R: int, steps: int, eos: int, power: float, use_graph: bool) -> list:
+    def _generate_beams(self, ids, own: np.ndarray, B: int, S: int, K: int, R: int, steps: int, eos: int, power: float, use_graph: bool) -> list:
         self.prefill(ids)
         d = self._decode_state(R)
         b = self._beam_state(d, B, K, eos)
-        # the prompt's pages stand in the first beam's row; the others take them over as children of it
+        # the prompt's pages (`own`: the block table) stand in the first beam's row; the others take them over as children of it
         book, held, whole = paged.PagePool(self.k_cache[0].shape[0]), -(-S // paged.PAGE), S // paged.PAGE
-        book.keep(self.page_table[:B, :held])
-        table = np.zeros((R, self.page_table.shape[1]), np.int32)
-        table[::K, :held] = self.page_table[:B, :held]
+        book.keep(own[:B, :held])
+        table = np.zeros((R, own.shape[1]), np.int32)
+        table[::K, :held] = own[:B, :held]
         if whole < held:
             table[np.arange(R) % K != 0, whole] = book.take(R - B)
         core._backend().upload(b["spare"]._handle, book.take(R))

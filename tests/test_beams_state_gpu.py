@@ -57,3 +57,20 @@ def test_searches_of_many_kinds_leave_nothing_behind(backend, collected):
     eng.generate_beams(ids, 4, STEPS, 5)
     assert np.array_equal(eng.generate(np.repeat(ids, 4, 0), 5), want), "the captured step of the plain generation is another one"
     eng.dispose()
+
+
+def test_the_prompts_pages_are_those_of_the_block_table_as_it_stands(backend):
+    """A program may give the sequences other pages; the array that an engine was built with is the program's own."""
+    pages = np.arange(16, dtype=np.int32).reshape(8, 2)
+    given = pages.copy()
+    eng = engine(page_table=given)
+    ids = synth.token_ids("beams.table", (2, 130), 512)
+    want = eng.generate_beams(ids, K, STEPS)
+    given[:] = pages[::-1]
+    assert eng.generate_beams(ids, K, STEPS) == want and np.array_equal(eng.block_table.dataAsync(), pages)
+    other = np.random.default_rng(3).permutation(16).astype(np.int32).reshape(8, 2)
+    backend.upload(eng.block_table._handle, other)
+    for use_graph in (True, False):
+        assert eng.generate_beams(ids, K, STEPS, use_graph=use_graph) == want
+        assert np.array_equal(eng.block_table.dataAsync(), other), "the table is left as it was"
+    eng.dispose()
