@@ -740,8 +740,8 @@ class Qwen3Engine(DecoderEngine):
         (B, S), K, R = ids.shape, int(beams), ids.shape[0] * int(beams)
         if not 1 <= K <= 32 or R > self.B or steps < 1 or S < 1:
             raise ValueError(f"{B} prompts of {S} tokens with {K} beams and {steps} steps: 1 to 32 beams, at most {self.B} in all, and one step at least")
-        if S + steps > self.max_seq_len:
-            raise ValueError(f"Cache overflow: {S} + {steps} positions, but maxSeqLen is {self.max_seq_len}")
+        if S + steps - 1 > self.max_seq_len:       # (the last token is not in the cache)
+            raise ValueError(f"Cache overflow: {S} + {steps - 1} positions, but maxSeqLen is {self.max_seq_len}")
         own = self.block_table.dataAsync()
         sampler, self.sampler = self.sampler, None
         try:

@@ -74,3 +74,16 @@ def test_the_prompts_pages_are_those_of_the_block_table_as_it_stands(backend):
         assert eng.generate_beams(ids, K, STEPS, use_graph=use_graph) == want
         assert np.array_equal(eng.block_table.dataAsync(), other), "the table is left as it was"
     eng.dispose()
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_a_search_fills_the_cache_to_its_last_position(backend, use_graph):
+    """As generate does: the last token's keys are not needed."""
+    eng, roomy = engine(room=128), engine(room=384)
+    ids = synth.token_ids("beams.full", (2, 117), 512)
+    assert eng.generate(ids, 12).shape == (2, 12)
+    assert eng.generate_beams(ids, K, 12, use_graph=use_graph) == roomy.generate_beams(ids, K, 12, use_graph=use_graph)
+    with pytest.raises(ValueError, match="overflow"):
+        eng.generate_beams(ids, K, 13)
+    eng.dispose()
+    roomy.dispose()
