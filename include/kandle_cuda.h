@@ -117,6 +117,9 @@ int kd_workspace_bytes(uint64_t* bytes_out);
  * buffer of kd_attention_decode_noalloc with `byte_value` (stream-ordered), so that a test can tell
  * a kernel that read a slot it never wrote (0xFF gives NaN patterns) from one that did not. */
 int kd_debug_fill_scratch(int byte_value);
+/* Test support, no counterpart in the reference: whether the library takes two views as having memory in common, where a call refuses
+ * outputs that share memory with what it reads.  Touches no device. */
+int kd_debug_views_meet(const kd_tensor* a, const kd_tensor* b, int* meet);
 /* Test support, no counterpart in the reference: which form the library would give a call on a GPU of `sms`
  * multiprocessors.  Touch no device.
  *   linear       width of the output tiles of kd_linear_bf16 and its relatives (heads_of_128: of
@@ -425,7 +428,9 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
 /* Attention of new tokens over a paged cache, sequences of any lengths side by side: portions of prompts, drafts to be verified and next
  * tokens in one call (no counterpart in the reference, whose cache is contiguous and whose causal mask begins at position 0;
  * per sequence it is `scaled_dot_product_attention` of the last rows of a causal mask, packages/model-utils/src/attention/gqa.ts:407-414).
- *   q, out       bf16 [tokens,Hq,D] (D 64 or 128; strides multiples of 8), Hq a multiple (up to 64 times) of Hkv.  out must not be q
+ *   q, out       bf16 [tokens,Hq,D] (D 64 or 128; strides multiples of 8), Hq a multiple (up to 64 times) of Hkv.  out shares no memory with
+ *                what is read: items of a call are written while the queries of others are still to be read.  (Views that lie within one
+ *                another's span, as heads of one buffer, need equal strides)
  *   scale        between 1e-6 and 1e6
  *   k_pool, v_pool  bf16 [pages,Hkv,128,D]; block_table int32 [B <= 65535, max_pages <= 2^18] (rows of any stride): entries behind a
  *                sequence's last page are not read

@@ -4,6 +4,8 @@
 // (packages/backend-webgpu/src/base/device.ts:95-176, base/storage.ts:60-243): storages are
 // refcounted, views share a storage, release at refcount 0 returns the block to a free list.
 // Everything is ordered on one stream, so a block can be reused as soon as it is released.
+#include <algorithm>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <unordered_map>
@@ -139,6 +141,57 @@ int tensor_ptr(const kd_tensor* t, void** out) {
                 (long long)lo, (long long)hi, (unsigned long long)s->bytes);
   *out = static_cast<char*>(s->ptr) + t->offset * esz;
   return KD_OK;
+}
+
+// Whether sum_i k_i step_i = delta for some lo_i <= k_i <= hi_i, the steps in falling order.
+struct ViewSteps {
+  int n = 0;
+  int64_t step[KD_MAX_DIMS], lo[KD_MAX_DIMS], hi[KD_MAX_DIMS], reach[KD_MAX_DIMS + 1];
+  bool gives(int64_t delta, int i = 0) const {
+    if (i == n) return delta == 0;
+    const int64_t s = step[i], rest = reach[i + 1];
+    // |delta - k s| <= rest
+    const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t from = std::max(lo[i], -floor_div(rest - delta, s)), to = std::min(hi[i], floor_div(delta + rest, s));
+    if (to - from >= 8) return true;            // views that overlap themselves many times: not gone into
+    for (int64_t k = from; k <= to; ++k)
+      if (gives(delta - k * s, i + 1)) return true;
+    return false;
+  }
+};
+
+bool views_meet(const kd_tensor* a, const kd_tensor* b) {
+  if (!a || !b || a->storage != b->storage) return false;
+  int64_t first[2], last[2];                    // bytes
+  const kd_tensor* both[2] = {a, b};
+  for (int v = 0; v < 2; ++v) {
+    const kd_tensor* t = both[v];
+    int64_t lo = t->offset, hi = t->offset;
+    for (int i = 0; i < t->ndim; ++i) {
+      if (t->shape[i] == 0) return false;
+      const int64_t span = (t->shape[i] - 1) * t->strides[i];
+      (span >= 0 ? hi : lo) += span;
+    }
+    first[v] = lo * dtype_size(t->dtype);
+    last[v] = (hi + 1) * dtype_size(t->dtype);
+  }
+  if (last[0] <= first[1] || last[1] <= first[0]) return false;
+  if (a->ndim != b->ndim || dtype_size(a->dtype) != dtype_size(b->dtype)) return true;
+  ViewSteps w;
+  int64_t delta = b->offset - a->offset;
+  for (int i = 0; i < a->ndim; ++i) {
+    const int64_t na = a->shape[i], nb = b->shape[i], s = na > 1 ? a->strides[i] : b->strides[i];
+    if (na > 1 && nb > 1 && a->strides[i] != b->strides[i]) return true;
+    if ((na == 1 && nb == 1) || s == 0) continue;
+    int64_t lo = -(nb - 1), hi = na - 1;
+    if (s < 0) { const int64_t t = lo; lo = -hi; hi = -t; }
+    int j = w.n++;
+    for (; j > 0 && w.step[j - 1] < std::abs(s); --j) { w.step[j] = w.step[j - 1]; w.lo[j] = w.lo[j - 1]; w.hi[j] = w.hi[j - 1]; }
+    w.step[j] = std::abs(s); w.lo[j] = lo; w.hi[j] = hi;
+  }
+  w.reach[w.n] = 0;
+  for (int i = w.n - 1; i >= 0; --i) w.reach[i] = w.reach[i + 1] + std::max(-w.lo[i], w.hi[i]) * w.step[i];
+  return w.gives(delta);
 }
 
 // Scratch buffers that were outgrown.  They are kept until kd_shutdown instead of being freed at
@@ -416,6 +469,12 @@ KD_API int kd_debug_fill_scratch(int byte_value) {
   Context& c = ctx();
   if (c.workspace) KD_CUDA_CHECK(cudaMemsetAsync(c.workspace, byte_value, c.workspace_bytes, c.stream));
   return attention_decode_static_fill(byte_value);
+}
+
+KD_API int kd_debug_views_meet(const kd_tensor* a, const kd_tensor* b, int* meet) {
+  if (!a || !b || !meet) return fail(KD_ERR_INVALID, "null argument");
+  *meet = views_meet(a, b) ? 1 : 0;
+  return KD_OK;
 }
 
 KD_API int kd_empty_cache(void) {

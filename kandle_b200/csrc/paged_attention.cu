@@ -24,6 +24,7 @@
 // Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 75 us, 5.1 TB/s, of which some 15 are the launch, the division,
 // the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 44 us; 4 x 2048 tokens on 6144 (32 on 8) 1000 us,
 // 960 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -1260,7 +1261,8 @@ KD_API int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const
   if (q_start) KD_TRY(tensor_ptr(q_start, &ps));
   KD_REQUIRE(((reinterpret_cast<uintptr_t>(pq) | reinterpret_cast<uintptr_t>(pk) | reinterpret_cast<uintptr_t>(pv) | reinterpret_cast<uintptr_t>(po)) & 15) == 0,
              "q, pools and out must be 16-byte aligned");
-  KD_REQUIRE(po != pq, "out must not be q");
+  for (const kd_tensor* t : {q, k_pool, v_pool, block_table, ctx_len, q_start})
+    KD_REQUIRE(!views_meet(out, t), "out must not share memory with what the call reads");
   p.q = static_cast<const __nv_bfloat16*>(pq); p.k = static_cast<const __nv_bfloat16*>(pk); p.v = static_cast<const __nv_bfloat16*>(pv);
   p.o = static_cast<__nv_bfloat16*>(po);
   p.table = static_cast<const int*>(pt); p.ctx = static_cast<const int*>(pc); p.q_start = static_cast<const int*>(ps);

@@ -1,0 +1,53 @@
+"""Operators of a paged cache and of beam search refuse outputs that lie over what they read, before anything is launched."""
+import numpy as np
+import pytest
+import torch
+
+from kandle_b200 import core, lib, paged
+from kandle_b200.core import Tensor
+from tests.paged_cases import attention_answer, attention_case
+from tests.test_paged_gpu import put
+
+pytestmark = pytest.mark.gpu
+
+
+def refused(call):
+    with pytest.raises(lib.KandleCudaError) as e:
+        call()
+    assert e.value.status == 1 and "share" in str(e.value)
+
+
+def test_attention_refuses_outputs_over_what_it_reads(backend):
+    T, H, G, D = 40, 8, 2, 64
+    row = core.zeros((T + 8, 3 * H, D), "bfloat16")
+    view = lambda first, head, strides=(3 * H * D, D, 1): row._view((T, H, D), strides, first * 3 * H * D + head * D)  # noqa: E731
+    k, v = (core.zeros((3, G, 128, D), "bfloat16") for _ in range(2))
+    table, keys, start = Tensor(np.array([[0, 1]], np.int32)), Tensor(np.array([200], np.int32)), Tensor(np.array([0, T], np.int32))
+    q = view(0, 0)
+    before = backend.launch_count()
+    for out in (q, view(1, 0), view(8, 0), view(0, H - 1), view(0, H, (3 * H * D, 2 * D, 1))):
+        refused(lambda: paged.attention(q, k, v, table, keys, q_start=start, out=out))
+    for pool in (k, v):
+        refused(lambda: paged.attention(q, k, v, table, keys, out=pool._view((T, H, D), (H * D, D, 1), 64 * D)))
+    assert backend.launch_count() == before
+    wide = core.zeros((T * H * D + 64,), "bfloat16")
+    ints = core.zeros((64,), "int32")
+    paged.attention(q, k, v, table, keys, q_start=start, out=wide._view((T, H, D), (H * D, D, 1), 64))
+    paged.attention(q, k, v, ints._view((1, 2), (2, 1), 0), ints._view((1,), (1,), 8), out=core.zeros((T, H, D), "bfloat16"))
+    backend.synchronize()
+
+
+def test_queries_and_outputs_may_be_heads_of_one_buffer(backend):
+    """A projection's row holds queries and, behind them or in turn with them, room for the outputs."""
+    H, G, D = 8, 2, 64
+    c = attention_case([3, 150], [300, 400], H, G, D, seed=11)
+    T = c["q"].shape[0]
+    want, tol = attention_answer(c)
+    for step, first in ((1, H), (2, 1)):
+        rows = torch.zeros(T, 2 * H, D, dtype=torch.bfloat16)
+        rows[:, :H * step:step] = c["q"]
+        t = put(rows)
+        q, out = (t._view((T, H, D), (2 * H * D, step * D, 1), at * D) for at in (0, first))
+        paged.attention(q, put(c["k"]), put(c["v"]), put(c["table"]), put(c["keys"]), q_start=put(c["start"]), scale=c["scale"], out=out)
+        assert ((torch.tensor(out.dataAsync()).double() - want).abs() <= tol).all()
+        assert np.array_equal(q.dataAsync(), c["q"].float().numpy())
