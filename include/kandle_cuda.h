@@ -463,7 +463,7 @@ int kd_kv_pages_fork(const kd_tensor* const* pools, int n_pools, const kd_tensor
 /* A step of beam search: logits fp32 [requests,beams,V] or [requests*beams,V] (evenly spaced rows), scores fp32 [requests,beams <= 32].
  * Candidate (j, i) is worth scores[j] + logits[j,i] - log sum exp(logits[j]); every candidate of a beam whose score or sum is not
  * finite is worth minus infinity.  The best `beams` candidates whose token is not eos (negative: none), best first: out_scores fp32 (may
- * be scores), parents int32 (their beam), tokens int64.  ended fp32 (or NULL): the value of (j, eos) where that is among the best
+ * be scores; else outputs share no memory with one another or with what is read), parents int32 (their beam), tokens int64.  ended fp32 (or NULL): the value of (j, eos) where that is among the best
  * `beams` of all candidates, else minus infinity.  Candidates of one beam are ordered by their logits; equal ones go by the lower
  * beam, then the lower token; where there are fewer candidates, the rest are minus infinity with beam and token 0.  Uses the library's
  * scratch. */

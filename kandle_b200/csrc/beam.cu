@@ -456,6 +456,12 @@ KD_API int kd_beam_select(const kd_tensor* logits, const kd_tensor* scores, int 
   void *px, *ps, *po, *pp, *pt, *pe = nullptr, *scratch;
   KD_TRY(tensor_ptr(logits, &px)); KD_TRY(tensor_ptr(scores, &ps)); KD_TRY(tensor_ptr(out_scores, &po)); KD_TRY(tensor_ptr(parents, &pp)); KD_TRY(tensor_ptr(tokens, &pt));
   if (ended) KD_TRY(tensor_ptr(ended, &pe));
+  // The block that joins a request reads its scores before it writes, and the logits are read by others meanwhile.
+  const kd_tensor* outs[4] = {out_scores, parents, tokens, ended};
+  for (int i = 0; i < 4; ++i) {
+    KD_REQUIRE(!views_meet(outs[i], logits) && (!views_meet(outs[i], scores) || (i == 0 && po == ps)), "outputs must not share memory with what the call reads (out_scores may be scores)");
+    for (int j = 0; j < i; ++j) KD_REQUIRE(!views_meet(outs[i], outs[j]), "outputs must not share memory with one another");
+  }
   if (B == 0) return KD_OK;
   BeamParams p{};
   p.logits = static_cast<const float*>(px);

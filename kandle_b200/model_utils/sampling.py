@@ -70,7 +70,7 @@ def beam_select(logits: Tensor, scores: Tensor, eos: int = -1, out=None):
     """One step of beam search for every request (kd_beam_select).  logits fp32 [requests, beams, V] (or [requests * beams, V]), scores
     fp32 [requests, beams]: the log-probability of each beam so far.  Returns (scores, parents, tokens, ended), each [requests, beams]:
     the best continuations that go on, best first (score, the beam that each continues, its token), and for every old beam the score with
-    which it ends here by `eos` if that is among the best as many as there are beams, else -inf.  out: tensors to write them to.
+    which it ends here by `eos` if that is among the best as many as there are beams, else -inf.  out: tensors to write them to (the scores' may be `scores`).
     The reference has greedy and sampled tokens only."""
     if out is None:
         shape = scores.shape

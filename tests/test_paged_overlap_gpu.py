@@ -51,3 +51,25 @@ def test_queries_and_outputs_may_be_heads_of_one_buffer(backend):
         paged.attention(q, put(c["k"]), put(c["v"]), put(c["table"]), put(c["keys"]), q_start=put(c["start"]), scale=c["scale"], out=out)
         assert ((torch.tensor(out.dataAsync()).double() - want).abs() <= tol).all()
         assert np.array_equal(q.dataAsync(), c["q"].float().numpy())
+
+
+def test_beam_select_refuses_outputs_over_what_it_reads(backend):
+    """The outputs of a request are written while others' logits are still read; only the scores may be updated in place."""
+    B, K, V = 3, 4, 300
+    logits, scores = core.zeros((B, K, V)), core.zeros((B, K))
+    outs = [core.zeros((B, K), t) for t in ("float32", "int32", "int64", "float32")]
+    r = lambda x: x._handle.ref() if x is not None else None  # noqa: E731
+    call = lambda s, *o: lib.call("kd_beam_select", r(logits), r(s), -1, *map(r, o))  # noqa: E731
+    wide = core.zeros((B * K + 8,))
+    part = lambda at: wide._view((B, K), (K, 1), at)  # noqa: E731
+    inside = logits._view((B, K), (K, 1), 40)
+    refused(lambda: call(scores, inside, *outs[1:]))
+    refused(lambda: call(scores, *outs[:3], inside))
+    refused(lambda: call(part(0), part(4), *outs[1:]))
+    refused(lambda: call(part(4), part(0), *outs[1:]))
+    refused(lambda: call(scores, *outs[:3], outs[0]))
+    refused(lambda: call(scores, *outs[:3], scores))
+    call(part(0), part(0), *outs[1:])
+    call(scores, scores, *outs[1:3], None)
+    call(part(0), *outs)
+    backend.synchronize()
