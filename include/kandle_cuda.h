@@ -446,8 +446,9 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
  * library's scratch (up to 60 MB, whatever the sizes): make the first call before a capture. */
 int kd_attention_paged(const kd_tensor* q, const kd_tensor* k_pool, const kd_tensor* v_pool, const kd_tensor* block_table,
                        const kd_tensor* ctx_len, const kd_tensor* q_start, int max_query, float scale, const kd_tensor* out);
-/* Copies page src[i] to page dst[i] in every pool (each [pages,Hkv,128,D] of any type, all alike; the 128 rows of a head side by side):
- * a prefix for a sequence that will write on, or pages moved together.  src, dst int32 [n <= 65536].  A pair whose dst is in the lists
+/* Copies page src[i] to page dst[i] in every pool (each [pages,Hkv,128,D] of any type, all alike; the 128 rows of a head side by side; no
+ * memory shared with the lists or one another): a prefix for a sequence that will write on, or pages moved together.  src, dst int32
+ * [n <= 65536].  A pair whose dst is in the lists
  * again is left out and reported (code 105), and one with a page outside the pools (103).  Lists of more than 4096 pairs use the
  * library's scratch. */
 int kd_kv_pages_copy(const kd_tensor* const* pools, int n_pools, const kd_tensor* src, const kd_tensor* dst);
@@ -463,8 +464,8 @@ int kd_kv_pages_fork(const kd_tensor* const* pools, int n_pools, const kd_tensor
 /* A step of beam search: logits fp32 [requests,beams,V] or [requests*beams,V] (evenly spaced rows), scores fp32 [requests,beams <= 32].
  * Candidate (j, i) is worth scores[j] + logits[j,i] - log sum exp(logits[j]); every candidate of a beam whose score or sum is not
  * finite is worth minus infinity.  The best `beams` candidates whose token is not eos (negative: none), best first: out_scores fp32 (may
- * be scores; else outputs share no memory with one another or with what is read), parents int32 (their beam), tokens int64.  ended fp32 (or NULL): the value of (j, eos) where that is among the best
- * `beams` of all candidates, else minus infinity.  Candidates of one beam are ordered by their logits; equal ones go by the lower
+ * be scores; else outputs share no memory with one another or with what is read), parents int32 (their beam), tokens int64.  ended fp32
+ * (or NULL): the value of (j, eos) where that is among the best `beams` of all candidates, else minus infinity.  Candidates of one beam are ordered by their logits; equal ones go by the lower
  * beam, then the lower token; where there are fewer candidates, the rest are minus infinity with beam and token 0.  Uses the library's
  * scratch. */
 int kd_beam_select(const kd_tensor* logits, const kd_tensor* scores, int eos, const kd_tensor* out_scores, const kd_tensor* parents,

@@ -143,6 +143,12 @@ __global__ void __launch_bounds__(256) kv_fork_copy_kernel(const __grid_constant
   copy_head(base + s * P.page_bytes, base + d * P.page_bytes, (*length % 128) * P.row_bytes);
 }
 
+// Pools are written while the lists and tables are read by other blocks.
+static int apart_from_pools(const kd_tensor* const* pools, int n_pools, const kd_tensor* t, const char* what) {
+  for (int i = 0; i < n_pools; ++i) KD_REQUIRE(!views_meet(pools[i], t), "%s must not share memory with a pool", what);
+  return KD_OK;
+}
+
 static int page_pools(const kd_tensor* const* pools, int first, int count, PagePools* P) {
   const kd_tensor* a = pools[first];
   for (int i = 0; i < count; ++i) {
@@ -184,6 +190,8 @@ KD_API int kd_kv_pages_copy(const kd_tensor* const* pools, int n_pools, const kd
   KD_TRY(tensor_ptr(dst, &pd));
   PagePools P;
   for (int a = 0; a < n_pools; a += KVP_POOLS) KD_TRY(page_pools(pools, a, n_pools - a < KVP_POOLS ? n_pools - a : KVP_POOLS, &P));
+  KD_TRY(apart_from_pools(pools, n_pools, src, "src"));
+  KD_TRY(apart_from_pools(pools, n_pools, dst, "dst"));
   if (n > KVP_CHECK && n_pools > 0) {
     KD_TRY(get_workspace(n, &known));
     KD_CUDA_CHECK(launch_ex(kv_pages_check_kernel, dim3((n + 255) / 256), dim3(256), 0, (const int*)ps, (const int*)pd, n, (uint8_t*)known, ctx().error_flag));
@@ -216,6 +224,12 @@ KD_API int kd_kv_pages_fork(const kd_tensor* const* pools, int n_pools, const kd
   KD_TRY(tensor_ptr(parents, &pp)); KD_TRY(tensor_ptr(block_table, &pt)); KD_TRY(tensor_ptr(spare, &ps)); KD_TRY(tensor_ptr(length, &pl));
   PagePools P;
   for (int a = 0; a < n_pools; a += KVP_POOLS) KD_TRY(page_pools(pools, a, n_pools - a < KVP_POOLS ? n_pools - a : KVP_POOLS, &P));
+  KD_TRY(apart_from_pools(pools, n_pools, parents, "parents"));
+  KD_TRY(apart_from_pools(pools, n_pools, block_table, "block_table"));
+  KD_TRY(apart_from_pools(pools, n_pools, spare, "spare"));
+  KD_TRY(apart_from_pools(pools, n_pools, length, "length"));
+  KD_REQUIRE(!views_meet(block_table, spare) && !views_meet(block_table, parents) && !views_meet(block_table, length) && !views_meet(spare, parents) && !views_meet(spare, length),
+             "block_table and spare must not share memory with one another or with what the call reads");
   if (B == 0) return KD_OK;
   KD_TRY(get_workspace(8 * (uint64_t)B * K, &moves));
   KD_CUDA_CHECK(launch_ex(kv_fork_table_kernel, dim3(B), dim3(256), 0, (const int*)pp, K, (int*)pt, (int64_t)block_table->strides[0], (int)block_table->shape[1], (int*)ps,

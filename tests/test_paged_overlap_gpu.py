@@ -73,3 +73,29 @@ def test_beam_select_refuses_outputs_over_what_it_reads(backend):
     call(scores, scores, *outs[1:3], None)
     call(part(0), *outs)
     backend.synchronize()
+
+
+def test_forks_and_copies_refuse_lists_and_tables_in_one_another(backend):
+    B, K = 2, 3
+    pools = [core.zeros((8, 2, 128, 64), "bfloat16") for _ in range(3)]
+    ints = core.zeros((200,), "int32")
+    part = lambda at, *shape: ints._view(shape, (shape[1], 1) if len(shape) == 2 else (1,), at)  # noqa: E731
+    parents, table, spare, length = (lambda: part(0, B, K)), (lambda: part(10, B * K, 4)), (lambda: part(40, B * K)), (lambda: part(50, 1))
+    call = lambda a, b, c, d, p=pools: paged.fork_pages(p, a, b, c, d)  # noqa: E731
+    refused(lambda: call(part(12, B, K), table(), spare(), length()))
+    refused(lambda: call(parents(), table(), part(33, B * K), length()))
+    refused(lambda: call(parents(), table(), spare(), part(33, 1)))
+    refused(lambda: call(part(41, B, K), table(), spare(), length()))
+    refused(lambda: call(parents(), table(), spare(), part(45, 1)))
+    both = core.zeros((8 * 2 * 128 * 32 + 8,), "int32")
+    pool = both._view((8, 2, 128, 32), (8192, 4096, 32, 1), 0)
+    over = lambda *shape: both._view(shape, (shape[1], 1) if len(shape) == 2 else (1,), 100)  # noqa: E731
+    for args in ((over(B, K), table(), spare(), length()), (parents(), over(B * K, 4), spare(), length()), (parents(), table(), over(B * K), length()), (parents(), table(), spare(), over(1))):
+        refused(lambda: call(*args, p=[pool]))
+    refused(lambda: paged.copy_pages([pool], over(2), part(60, 2)))
+    refused(lambda: paged.copy_pages([pool], part(60, 2), over(2)))
+    call(parents(), table(), spare(), length())
+    paged.copy_pages([pool], both._view((2,), (1,), 8 * 8192), part(60, 2))
+    paged.copy_pages(pools, part(70, 0), part(60, 0))
+    with pytest.raises(lib.KandleCudaError, match="error code 105"):      # (two pairs 0 -> 0)
+        backend.synchronize()
