@@ -441,7 +441,8 @@ KD_API int kd_beam_select(const kd_tensor* logits, const kd_tensor* scores, int 
   const int64_t B = scores->shape[0], K = scores->shape[1];
   KD_REQUIRE(logits->dtype == KD_F32 && logits->ndim >= 2 && logits->ndim <= 3, "logits must be fp32 [requests, beams, V] or [requests x beams, V]");
   const int last = logits->ndim - 1;
-  const int64_t V = logits->shape[last], ld = logits->strides[last - 1];
+  // from one row to the next (the stride of a dimension of one is none)
+  const int64_t V = logits->shape[last], ld = logits->strides[logits->ndim == 3 && K == 1 ? 0 : last - 1];
   if (logits->ndim == 3)
     KD_REQUIRE(logits->shape[0] == B && logits->shape[1] == K && (logits->strides[0] == K * ld || B <= 1), "logits must hold evenly spaced rows, one for each of %lld x %lld beams", (long long)B, (long long)K);
   else
