@@ -361,8 +361,8 @@ class Qwen3Engine(DecoderEngine):
         the memory of the activations."""
         if portion is not None and portion < 1:
             raise ValueError(f"portions of {portion} tokens")
-        if portion is not None and portion < ids.shape[1]:
-            B, S = ids.shape
+        B, S = ids.shape if isinstance(ids, Tensor) else np.shape(ids)
+        if portion is not None and portion < S:
             if S > self.max_seq_len:
                 raise ValueError(f"prefill of {B}x{S} exceeds the engine's {self.B}x{self.max_seq_len}")
             host = ids.dataAsync() if isinstance(ids, Tensor) else np.asarray(ids)
@@ -375,6 +375,10 @@ class Qwen3Engine(DecoderEngine):
         """The next tokens ids [B,S] of the running sequences, whose cache holds self.pos positions: the rest of a prompt, or what a user
         says next (a token that decode_step has just returned is not in the cache yet and comes first).  Returns what prefill does.
         Each new token attends to everything before it (kd_attention_paged with a paged cache)."""
+        if not isinstance(ids, Tensor):
+            ids = np.ascontiguousarray(ids, dtype=np.int32)
+        if len(ids.shape) != 2 or 0 in ids.shape:
+            raise ValueError(f"tokens of shape {tuple(ids.shape)}: at least one for each sequence [B,S] is needed")
         if self.pos and ids.shape[0] != self.cur_B:
             raise ValueError(f"{ids.shape[0]} token rows for {self.cur_B} running sequences")
         if self.pos + ids.shape[1] > self.max_seq_len:

@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from kandle_b200 import lib, synth
+from kandle_b200.core import Tensor
 from kandle_b200.engine import Qwen3Engine
 from kandle_b200.model_utils.qwen3 import Qwen3Config
 
@@ -51,4 +52,20 @@ def test_only_the_last_portion_goes_through_the_vocabulary(backend):
         eng.extend(ids[:, 48:])
 
     assert two < one + launches(behind)
+    eng.dispose()
+
+
+def test_tokens_come_as_lists_arrays_or_tensors(backend):
+    """As prefill has always taken them; no token at all is refused, and nothing has changed then."""
+    eng = engine(paged=True)
+    ids = synth.token_ids("portions.lists", (2, 50), 1024)
+    want = eng.prefill(ids[:, :30], all_logits=True)[1].dataAsync()
+    behind = eng.extend(ids[:, 30:], all_logits=True)[1].dataAsync()
+    for kind in (lambda a: a.tolist(), lambda a: a.astype(np.int64), lambda a: Tensor(np.ascontiguousarray(a, np.int32))):
+        assert np.array_equal(eng.prefill(kind(ids[:, :30]), all_logits=True)[1].dataAsync(), want)
+        for none in (ids[:, :0], [[], []], ids[0]):
+            with pytest.raises(ValueError, match="at least one"):
+                eng.extend(none)
+        assert np.array_equal(eng.extend(kind(ids[:, 30:]), all_logits=True)[1].dataAsync(), behind) and eng.pos == 50
+        assert np.array_equal(eng.prefill(kind(ids), all_logits=True, portion=30)[1].dataAsync(), np.concatenate([want, behind], 1))
     eng.dispose()
