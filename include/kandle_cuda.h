@@ -431,7 +431,7 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
  *   q, out       bf16 [tokens,Hq,D] (D 64 or 128; strides multiples of 8), Hq a multiple (up to 64 times) of Hkv.  out shares no memory with
  *                what is read: items of a call are written while the queries of others are still to be read.  (Views that lie within one
  *                another's span, as heads of one buffer, need equal strides)
- *   scale        between 1e-6 and 1e6
+ *   scale        between 1e-6 and 1e6.  (Scores of -1e30 and less, before or after it, are not told from hidden ones)
  *   k_pool, v_pool  bf16 [pages,Hkv,128,D]; block_table int32 [B <= 65535, max_pages <= 2^18] (rows of any stride): entries behind a
  *                sequence's last page are not read
  *   ctx_len      int32 [B], or one number for all: the keys of sequence b, its new tokens' included (they are the last ones)

@@ -22,8 +22,8 @@
 // without a row have no exponentials (32 single tokens: 84.1 us with a row's 128 scores in straight code, 80.3 in loops, 75.0 so).
 //
 // Measured: 32 single tokens on up to 6000 positions (16 heads on 8 of 128, 379 MB) 75 us, 5.1 TB/s, of which some 15 are the launch, the division,
-// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 44 us; 4 x 2048 tokens on 6144 (32 on 8) 1000 us,
-// 960 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
+// the blocks' change from one item to the next and the joins; 8 x 9 tokens on 9000 (32 on 8, 153 MB) 44 us; 4 x 2048 tokens on 6144 (32 on 8) 1015 us (1000 to
+// 1030 from one machine to another), 948 TFLOP/s: a step of 3700 cycles, in which a softmax takes 3000 (load 440, maximum 450, exponentials 1800, store 400) and waits 600 for its S.
 #include <initializer_list>
 #include <type_traits>
 
