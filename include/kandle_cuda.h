@@ -429,8 +429,8 @@ int kd_attention_decode_paged(const kd_tensor* q, const kd_tensor* k_pool, const
  * tokens in one call (no counterpart in the reference, whose cache is contiguous and whose causal mask begins at position 0;
  * per sequence it is `scaled_dot_product_attention` of the last rows of a causal mask, packages/model-utils/src/attention/gqa.ts:407-414).
  *   q, out       bf16 [tokens,Hq,D] (D 64 or 128; strides multiples of 8), Hq a multiple (up to 64 times) of Hkv.  out shares no memory with
- *                what is read: items of a call are written while the queries of others are still to be read.  (Views that lie within one
- *                another's span, as heads of one buffer, need equal strides)
+ *                what is read: items of a call are written while the queries of others are still to be read.  (Large views that lie within
+ *                one another's span, as heads of one buffer, need equal strides)
  *   scale        between 1e-6 and 1e6.  (Scores of -1e30 and less, before or after it, are not told from hidden ones)
  *   k_pool, v_pool  bf16 [pages,Hkv,128,D]; block_table int32 [B <= 65535, max_pages <= 2^18] (rows of any stride): entries behind a
  *                sequence's last page are not read

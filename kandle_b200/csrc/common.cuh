@@ -72,8 +72,8 @@ int get_workspace(uint64_t bytes, void** out);
 int tensor_ptr(const kd_tensor* t, void** out);
 int storage_lookup(uint64_t handle, Storage** out);
 // Whether two views (null: none) have memory in common, for calls whose blocks read one while others write the other.  Views that lie within
-// one another's span of memory but not in one another (heads of one buffer in turn) are told apart if type, rank and strides agree; else
-// the spans decide.
+// one another's span of memory but not in one another (heads of one buffer in turn) are told apart if rank and strides agree or one of them has
+// no more than 4096 elements; else the spans decide.
 bool views_meet(const kd_tensor* a, const kd_tensor* b);
 
 __host__ __device__ inline int dtype_size(int dt) {

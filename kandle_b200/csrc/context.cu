@@ -143,17 +143,28 @@ int tensor_ptr(const kd_tensor* t, void** out) {
   return KD_OK;
 }
 
-// Whether sum_i k_i step_i = delta for some lo_i <= k_i <= hi_i, the steps in falling order.
+// Whether sum_i k_i step_i = delta for some lo_i <= k_i <= hi_i.
 struct ViewSteps {
   int n = 0;
-  int64_t step[KD_MAX_DIMS], lo[KD_MAX_DIMS], hi[KD_MAX_DIMS], reach[KD_MAX_DIMS + 1];
+  int64_t step[KD_MAX_DIMS + 1], lo[KD_MAX_DIMS + 1], hi[KD_MAX_DIMS + 1], reach[KD_MAX_DIMS + 2];
+  void add(int64_t s, int64_t from, int64_t to) {                    // steps in falling order
+    if (s == 0 || (from == 0 && to == 0)) return;
+    if (s < 0) { const int64_t t = from; from = -to; to = -t; s = -s; }
+    int j = n++;
+    for (; j > 0 && step[j - 1] < s; --j) { step[j] = step[j - 1]; lo[j] = lo[j - 1]; hi[j] = hi[j - 1]; }
+    step[j] = s; lo[j] = from; hi[j] = to;
+  }
+  void close() {
+    reach[n] = 0;
+    for (int i = n - 1; i >= 0; --i) reach[i] = reach[i + 1] + std::max(-lo[i], hi[i]) * step[i];
+  }
   bool gives(int64_t delta, int i = 0) const {
     if (i == n) return delta == 0;
     const int64_t s = step[i], rest = reach[i + 1];
     // |delta - k s| <= rest
     const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
     const int64_t from = std::max(lo[i], -floor_div(rest - delta, s)), to = std::min(hi[i], floor_div(delta + rest, s));
-    if (to - from >= 8) return true;            // views that overlap themselves many times: not gone into
+    if (to - from >= 16) return true;           // views that overlap themselves many times: not gone into
     for (int64_t k = from; k <= to; ++k)
       if (gives(delta - k * s, i + 1)) return true;
     return false;
@@ -162,36 +173,41 @@ struct ViewSteps {
 
 bool views_meet(const kd_tensor* a, const kd_tensor* b) {
   if (!a || !b || a->storage != b->storage) return false;
-  int64_t first[2], last[2];                    // bytes
-  const kd_tensor* both[2] = {a, b};
-  for (int v = 0; v < 2; ++v) {
-    const kd_tensor* t = both[v];
-    int64_t lo = t->offset, hi = t->offset;
+  if (numel(b) < numel(a)) std::swap(a, b);
+  const int64_t za = dtype_size(a->dtype), zb = dtype_size(b->dtype), delta = b->offset * zb - a->offset * za;      // (in bytes, all of them)
+  const auto span = [](const kd_tensor* t, int64_t z, int64_t& first, int64_t& last) {
+    first = t->offset * z;
+    last = first + z;
     for (int i = 0; i < t->ndim; ++i) {
-      if (t->shape[i] == 0) return false;
-      const int64_t span = (t->shape[i] - 1) * t->strides[i];
-      (span >= 0 ? hi : lo) += span;
+      const int64_t reach = (t->shape[i] - 1) * t->strides[i] * z;
+      (reach >= 0 ? last : first) += reach;
     }
-    first[v] = lo * dtype_size(t->dtype);
-    last[v] = (hi + 1) * dtype_size(t->dtype);
-  }
-  if (last[0] <= first[1] || last[1] <= first[0]) return false;
-  if (a->ndim != b->ndim || dtype_size(a->dtype) != dtype_size(b->dtype)) return true;
+  };
+  int64_t first_a, last_a, first_b, last_b;
+  if (numel(a) == 0) return false;
+  span(a, za, first_a, last_a);
+  span(b, zb, first_b, last_b);
+  if (last_a <= first_b || last_b <= first_a) return false;
+  bool alike = a->ndim == b->ndim;
+  for (int i = 0; alike && i < a->ndim; ++i) alike = a->shape[i] == 1 || b->shape[i] == 1 || a->strides[i] * za == b->strides[i] * zb;
   ViewSteps w;
-  int64_t delta = b->offset - a->offset;
-  for (int i = 0; i < a->ndim; ++i) {
-    const int64_t na = a->shape[i], nb = b->shape[i], s = na > 1 ? a->strides[i] : b->strides[i];
-    if (na > 1 && nb > 1 && a->strides[i] != b->strides[i]) return true;
-    if ((na == 1 && nb == 1) || s == 0) continue;
-    int64_t lo = -(nb - 1), hi = na - 1;
-    if (s < 0) { const int64_t t = lo; lo = -hi; hi = -t; }
-    int j = w.n++;
-    for (; j > 0 && w.step[j - 1] < std::abs(s); --j) { w.step[j] = w.step[j - 1]; w.lo[j] = w.lo[j - 1]; w.hi[j] = w.hi[j - 1]; }
-    w.step[j] = std::abs(s); w.lo[j] = lo; w.hi[j] = hi;
+  if (alike) {
+    for (int i = 0; i < a->ndim; ++i) w.add(a->shape[i] > 1 ? a->strides[i] * za : b->strides[i] * zb, -(b->shape[i] - 1), a->shape[i] - 1);
+    w.add(1, -(zb - 1), za - 1);
+    w.close();
+    return w.gives(delta);
   }
-  w.reach[w.n] = 0;
-  for (int i = w.n - 1; i >= 0; --i) w.reach[i] = w.reach[i + 1] + std::max(-w.lo[i], w.hi[i]) * w.step[i];
-  return w.gives(delta);
+  // other layouts: each element of the smaller view, if they are few
+  if (numel(a) > 4096) return true;
+  for (int i = 0; i < b->ndim; ++i) w.add(b->strides[i] * zb, -(b->shape[i] - 1), 0);
+  w.add(1, -(zb - 1), za - 1);
+  w.close();
+  for (int64_t e = 0; e < numel(a); ++e) {
+    int64_t at = 0, left = e;
+    for (int i = a->ndim - 1; i >= 0; --i) { at += left % a->shape[i] * a->strides[i] * za; left /= a->shape[i]; }
+    if (w.gives(delta - at)) return true;
+  }
+  return false;
 }
 
 // Scratch buffers that were outgrown.  They are kept until kd_shutdown instead of being freed at

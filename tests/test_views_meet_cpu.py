@@ -68,3 +68,39 @@ def test_views_of_equal_strides_against_their_elements(seed):
         assert meet(a, b) == want == meet(b, a)
         both[want] += 1
     assert min(both) > 200
+
+
+def bytes_of(t):
+    size = {F32: 4, BF16: 2}[t.dtype]
+    return {e * size + i for e in elements(t) for i in range(size)}
+
+
+def test_a_small_view_in_the_gaps_of_another():
+    """A row's padding holds something else: one number, a short list, of another type or rank."""
+    table = view((50, 6), (10, 1), 0, F32)
+    for at in (6, 9, 26, 496):
+        assert not meet(table, view((1,), (1,), at, F32)) and not meet(view((1, 2), (2, 1), at - at % 10 + 6, F32), table)
+    assert meet(table, view((1,), (1,), 25, F32)) and meet(table, view((2,), (1,), 9, F32)) and not meet(table, view((40,), (10,), 7, F32))
+    assert not meet(table, view((8,), (1,), 12)) and meet(table, view((9,), (1,), 12)) and not meet(view((2, 3), (20, 1), 13), table)
+    assert meet(view((70, 80), (200, 2)), view((80, 70), (2, 201), 1)), "large and unlike: the spans decide"
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_small_views_of_any_strides_against_their_bytes(seed):
+    rng = np.random.default_rng(seed)
+    both = [0, 0]
+    for _ in range(1500):
+        pair = []
+        for _ in range(2):
+            dims, inner, strides, shape = int(rng.integers(1, 4)), 1, [], []
+            for _ in range(dims):
+                strides.append(inner * int(rng.integers(1, 4)) * (1 if rng.random() < 0.8 else -1))
+                shape.append(int(rng.integers(1, 5)))
+                inner = abs(strides[-1]) * int(rng.integers(1, 6))
+            dtype = F32 if rng.random() < 0.5 else BF16
+            pair.append(view(shape, strides, (250 if dtype == F32 else 500) + int(rng.integers(-30, 31)), dtype))
+        a, b = pair
+        want = bool(bytes_of(a) & bytes_of(b))
+        assert meet(a, b) == want == meet(b, a)
+        both[want] += 1
+    assert min(both) > 200
