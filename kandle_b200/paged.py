@@ -41,7 +41,8 @@ def attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tensor, ct
               scale: float | None = None, out: Tensor | None = None) -> Tensor:
     """Attention of new tokens over a paged cache (kd_attention_paged).  q [tokens, Hq, D]: sequence b's new tokens are the rows
     q_start[b] .. q_start[b+1] (without q_start: equal shares), their keys and values already the last of its ctx_len[b] positions in the
-    pages; each sees the positions up to its own.  max_query: the most new tokens of a sequence, if the program knows it."""
+    pages; each sees the positions up to its own.  max_query: the most new tokens of a sequence, if the program knows it.  out shares no memory with
+    what is read; its rows outside the sequences stay as they are (without `out` they hold anything)."""
     if out is None:
         out = Tensor(_handle=core._output(q.shape, q.dtype))
     lib.call("kd_attention_paged", _r(q), _r(k_pool), _r(v_pool), _r(block_table), _r(ctx_len), _r(q_start), int(max_query),
